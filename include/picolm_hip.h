@@ -359,6 +359,165 @@ int plh_forward(const plh_model *m, int token, int pos, void *workspace, float *
 int plh_forward_prefill(const plh_model *m, const int *tokens, int n_tokens, int start_pos,
                         void *workspace, float *logits, float *x_out);
 
+/* ---- rotary positions: scaled tables, part of a head ------------------------ */
+/* What model.c:545-556 and tensor.c:531-603 lack for models trained with
+ * scaled frequencies or a partly rotated head.  A pair i < rot_dim/2 turns by
+ * theta_i per position, theta_i = freq_base^(-2i/rot_dim) changed by
+ *   NONE    nothing
+ *   LINEAR  theta / factor
+ *   NTK     freq_base * factor^(rot_dim/(rot_dim-2)) in freq_base's place
+ *           (rot_dim > 2)
+ *   BANDS   by the turns t = trained_len * theta / 2pi within the trained
+ *           context: with s = clamp((t - low)/(high - low), 0, 1),
+ *           (1-s) theta/factor + s theta
+ *   RAMP    by the pair's number: with d(t) = rot_dim ln(trained_len/(2pi t)) /
+ *           (2 ln freq_base), lo = max(0, floor d(high)), hi = min(rot_dim-1,
+ *           ceil d(low)), g = clamp((i-lo)/max(hi-lo, 1e-3), 0, 1),
+ *           theta (1-g) + theta/factor g; cos and sin are then also
+ *           multiplied by `magnitude`
+ * magnitude 0 stands for 1, with RAMP for 0.1 ln factor + 1. */
+#define PLH_ROPE_SCALE_NONE 0
+#define PLH_ROPE_SCALE_LINEAR 1
+#define PLH_ROPE_SCALE_NTK 2
+#define PLH_ROPE_SCALE_BANDS 3
+#define PLH_ROPE_SCALE_RAMP 4
+typedef struct {
+    int rot_dim; /* even, 2..256: the rotated elements of a head, its first ones */
+    int scaling;
+    double freq_base, factor;
+    double trained_len, low, high; /* BANDS and RAMP */
+    double magnitude;
+} plh_rope_spec;
+/* theta_i into freq[rot_dim/2] and the magnitude into *magnitude (host; no
+ * device needed).  -1 for a specification outside the above. */
+int plh_rope_frequencies_host(const plh_rope_spec *spec, double *freq, double *magnitude);
+/* cos and sin of positions first_pos..first_pos+n_pos-1, device arrays
+ * [n_pos][rot_dim/2]: angle, reduction and functions in 64 bits, rounded once
+ * (positions up to 2^31-1).  With rot_dim = head_dim they are also what
+ * plh_attn_* and plh_forward* take as rope_cos / rope_sin. */
+int plh_rope_tables(const plh_rope_spec *spec, int first_pos, int n_pos, float *cos_tab,
+                    float *sin_tab);
+
+/* Tables as the rotations below read them: device [n_pos][rot_dim/2], row p
+ * for position p.  rope_type PLH_ROPE_LLAMA pairs (2i, 2i+1), PLH_ROPE_QWEN
+ * pairs (i, i + rot_dim/2); elements from rot_dim on stay as they are. */
+typedef struct {
+    int rope_type, rot_dim, n_pos;
+    const float *cos_tab, *sin_tab;
+} plh_rope;
+/* Rotates n_rows rows of q (n_heads heads) and of k (n_kv_heads heads; either
+ * may have 0 heads), row r at position pos[r] (device): each head is
+ * head_dim floats (even, up to 256, rot_dim at most head_dim), a row's heads
+ * lie next to each other and rows *_stride floats apart.  An output may be
+ * its input (same pointer and stride); other overlaps are not allowed.
+ * Outputs are the 64-bit rotation rounded once; rows at a position outside
+ * the tables get NaN in their rotated elements. */
+int plh_rope_rows(const plh_rope *rope, int n_rows, const int32_t *pos, int head_dim,
+                  const float *q, int n_heads, int q_stride, float *q_out, int q_out_stride,
+                  const float *k, int n_kv_heads, int k_stride, float *k_out, int k_out_stride);
+
+/* ---- paged 8-bit KV cache ---------------------------------------------------- */
+/* K and V of several sequences in half of the fp16 cache's bytes.  A block is
+ * 32 tokens of one kv head; its k and its v are int8 codes with one fp32
+ * scale each, value = code * scale.  A page is page_tokens tokens (a multiple
+ * of 32) of every layer and head:
+ *     codes  int8  [n_pages][n_layers][n_kv_heads][page_tokens/32][2][Dp/32][1024]
+ *     scales float [n_pages][n_layers][n_kv_heads][page_tokens/32][2]
+ * ([2]: k, v; Dp = head_dim rounded up to 32).  A 1024-byte tile is 32 tokens
+ * x 32 elements in matrix-core operand order: byte 256 g + 16 i + 8 h + j holds
+ *     k: token 16 h + i,             element 8 g + j
+ *     v: token 16 (j/4) + 4 g + j%4, element 16 h + i
+ * of the tile.  Scales are not negative.  A token's place in a block is its
+ * position modulo 32.
+ *
+ * Limits: head_dim even, 2..256; up to 1024 sequences; a page's codes below
+ * 2 GiB; max_pages * page_tokens below 2^30.  codes is 16-byte aligned, the
+ * other arrays naturally.  The calls below return -1 (plh_last_error) for
+ * descriptors outside this. */
+typedef struct {
+    int n_layers, n_kv_heads, head_dim;
+    int n_pages, page_tokens;
+    int8_t *codes;  /* device, plh_kv8_code_bytes */
+    float *scales;  /* device, plh_kv8_scale_bytes */
+} plh_kv8_cache;
+/* The sequences that live in a cache: row s of table lists the pages of
+ * sequence s, of which the first ceil(len[s]/page_tokens) count (-1 behind
+ * them); refs[p] is how many rows list page p (0: free).  All device memory,
+ * zero-filled (table with -1) to start. */
+typedef struct {
+    int n_seqs, max_pages;
+    int32_t *table; /* [n_seqs][max_pages] */
+    int32_t *len;   /* [n_seqs] tokens */
+    int32_t *refs;  /* [n_pages] */
+} plh_kv8_seqs;
+/* Bytes of codes and scales; 0 for a cache outside the limits. */
+size_t plh_kv8_code_bytes(const plh_kv8_cache *cache);
+size_t plh_kv8_scale_bytes(const plh_kv8_cache *cache);
+
+/* Page operations.  Each is one vector over the sequences (device int32
+ * [n_seqs]), queued like the other calls and fit for graph capture; table,
+ * len and refs are as described above before and after.
+ *
+ * trim: len[s] = keep[s] where 0 <= keep[s] < len[s]; pages behind it are
+ * given back (keep[s] = 0 frees the sequence; other values leave it).
+ * fork: sequence s becomes what parent[s] was before the call (0 <= parent[s] <
+ * n_seqs, parent[s] != s; other values leave it): its own pages are given
+ * back, the parent's are shared.  Any mapping, permutations included.
+ * extend: room for add[s] > 0 more tokens, len[s] += add[s].  New pages are the
+ * free ones of the lowest numbers, handed out in sequence order, and a
+ * sequence whose last page is partly filled and still shared first gets a
+ * copy of it (every layer).  status (device int32 [2]) becomes {0, 0}; when
+ * {pages short, 0} or {.., 1 + first sequence whose table row is too short}
+ * nothing was changed.
+ * compact: the n live pages move to numbers 0..n-1 (the live pages from n on
+ * to the free places below n, both in rising order), tables follow.  status
+ * becomes {n, pages moved}. */
+int plh_kv8_trim(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, const int32_t *keep);
+int plh_kv8_fork(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, const int32_t *parent);
+int plh_kv8_extend(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, const int32_t *add,
+                   int32_t *status);
+int plh_kv8_compact(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, int32_t *status);
+
+/* The rows of a batch: sequence s has rows row_start[s]..row_start[s+1]-1 of
+ * n_rows (row_start: device, [n_seqs+1], rising; rows from row_start[n_seqs] on
+ * are not touched), which are its LAST tokens: with m rows, row i of them is
+ * the token at position len[s] - m + i.
+ *
+ * append: stores k and v rows (n_kv_heads*head_dim floats each, k_stride and
+ * v_stride floats apart) of layer `layer`, after plh_kv8_extend has made their
+ * room.  With `rope` (NULL: k is stored as it is) k is rotated to the row's
+ * position first, and with n_heads > 0 the q rows likewise into q_out (which
+ * may be q, same stride), both as plh_rope_rows rounds them.  Quantisation,
+ * per block and for k and v alone: s = max(|x| of the call's rows) / 127;
+ * where older rows lie before them in the block, s = max(s, the block's
+ * scale), and if that grew, the block's codes become round(code * old / s).
+ * New codes are round(x / s) (64-bit quotients, ties to even), 0 where s = 0.
+ * A block begun by the call starts from zeroed codes.  Rows that are not
+ * finite make their block's scale NaN (until a call begins the block again),
+ * so that nothing that attends over it passes for a result.  Rows whose page
+ * is missing or shared (refs != 1), and rows before position 0, are dropped.
+ * Calls with the same rows again store the same. */
+int plh_kv8_append(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, int layer, int n_rows,
+                   const int32_t *row_start, const plh_rope *rope, const float *q, int n_heads,
+                   int q_stride, float *q_out, int q_out_stride, const float *k, int k_stride,
+                   const float *v, int v_stride);
+/* Attention of every row (n_heads heads of head_dim floats, a multiple of
+ * n_kv_heads; already rotated) over its sequence's tokens at positions up to
+ * its own, scores scaled by 1/sqrt(head_dim), in one launch for any mixture of
+ * single tokens and prompts.  Weights and sums in fp32; q and the weights
+ * enter the matrix cores as two fp16 parts (22 bits).  A row before position 0
+ * gets zeros; a row whose keys lie on a page number outside the cache, or in a
+ * block whose scale is NaN, gets NaN.  out must not overlap q.  The partial
+ * results of long sequences split over workgroups use the library workspace;
+ * the first call of a head size allocates it. */
+int plh_kv8_attn(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, int layer, int n_heads,
+                 int n_rows, const int32_t *row_start, const float *q, int q_stride, float *out,
+                 int out_stride);
+/* The rows' stored values (code * scale) into k and v.  Rows before position
+ * 0 give zeros, rows on a page number outside the cache NaN. */
+int plh_kv8_fetch(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, int layer, int n_rows,
+                  const int32_t *row_start, float *k, int k_stride, float *v, int v_stride);
+
 /* Tuning knobs (bench sweeps).  key 1: decode target workgroups per launch
  * (0 = default); key 2: decode contexts of at most this many positions are
  * not split (multiple of 128, 0 = default); key 3: GEMV rows per thread

@@ -55,6 +55,27 @@ class PlhModel(C.Structure):
                 ("layers", C.POINTER(PlhLayer))]
 
 
+class PlhRopeSpec(C.Structure):
+    _fields_ = [("rot_dim", C.c_int), ("scaling", C.c_int), ("freq_base", C.c_double),
+                ("factor", C.c_double), ("trained_len", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("magnitude", C.c_double)]
+
+
+class PlhRope(C.Structure):
+    _fields_ = [("rope_type", C.c_int), ("rot_dim", C.c_int), ("n_pos", C.c_int),
+                ("cos_tab", _vp), ("sin_tab", _vp)]
+
+
+class PlhKv8Cache(C.Structure):
+    _fields_ = [("n_layers", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("n_pages", C.c_int), ("page_tokens", C.c_int), ("codes", _vp), ("scales", _vp)]
+
+
+class PlhKv8Seqs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("max_pages", C.c_int), ("table", _vp), ("len", _vp),
+                ("refs", _vp)]
+
+
 _SIGS = {
     # lifecycle
     "plh_init": (_i, [_i]),
@@ -113,6 +134,20 @@ _SIGS = {
     "plh_forward_workspace_bytes": (_sz, [C.POINTER(PlhModel)]),
     "plh_forward": (_i, [C.POINTER(PlhModel), _i, _i, _vp, _vp, _vp]),
     "plh_forward_prefill": (_i, [C.POINTER(PlhModel), _vp, _i, _i, _vp, _vp, _vp]),
+    # rotary positions: scaled tables, part of a head
+    "plh_rope_frequencies_host": (_i, [_vp, _vp, _vp]),
+    "plh_rope_tables": (_i, [_vp, _i, _i, _vp, _vp]),
+    "plh_rope_rows": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i]),
+    # paged 8-bit KV cache
+    "plh_kv8_code_bytes": (_sz, [_vp]),
+    "plh_kv8_scale_bytes": (_sz, [_vp]),
+    "plh_kv8_trim": (_i, [_vp] * 3),
+    "plh_kv8_fork": (_i, [_vp] * 3),
+    "plh_kv8_extend": (_i, [_vp] * 4),
+    "plh_kv8_compact": (_i, [_vp] * 3),
+    "plh_kv8_append": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i]),
+    "plh_kv8_attn": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _i]),
+    "plh_kv8_fetch": (_i, [_vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i]),
     "plh_set_tuning": (_i, [_i, _i]),
 }
 

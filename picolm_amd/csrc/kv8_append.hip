@@ -1,0 +1,507 @@
+// kv8_append.hip -- rows into the paged 8-bit cache and back as values
+// (include/picolm_hip.h, plh_kv8_append and plh_kv8_fetch).
+#include <limits.h>
+#include <math.h>
+
+#include "attn_common.h"
+#include "kv8.h"
+
+namespace plh {
+
+int kv_check(const plh_kv8_cache* c, const plh_kv8_seqs* s, const char* what) {
+  if (!c || !s) {
+    set_error("%s: no cache or no sequences", what);
+    return -1;
+  }
+  if (plh_kv8_code_bytes(c) == 0) {
+    set_error("%s: a cache of %d layers, %d kv heads of %d, %d pages of %d tokens is not built",
+              what, c->n_layers, c->n_kv_heads, c->head_dim, c->n_pages, c->page_tokens);
+    return -1;
+  }
+  if (!c->codes || !c->scales || ((uintptr_t)c->codes & 15) || ((uintptr_t)c->scales & 3)) {
+    set_error("%s: codes (16-byte aligned) or scales are missing", what);
+    return -1;
+  }
+  if (s->n_seqs < 1 || s->n_seqs > kKvMaxSeqs || s->max_pages < 1 ||
+      (int64_t)s->max_pages * c->page_tokens >= (1 << 30)) {
+    set_error("%s: %d sequences (1..%d) of %d pages of %d tokens (below 2^30 in all)", what,
+              s->n_seqs, kKvMaxSeqs, s->max_pages, c->page_tokens);
+    return -1;
+  }
+  if (!s->table || !s->len || !s->refs) {
+    set_error("%s: table, len or refs is null", what);
+    return -1;
+  }
+  return 0;
+}
+
+int kv_ready(const char* what) {
+  if (ctx().stream) return 0;
+  set_error("%s: library not initialised", what);
+  return -1;
+}
+
+int kv_view(const plh_kv8_cache* c, const plh_kv8_seqs* s, int layer, int n_rows,
+            const int32_t* row_start, const char* what, KvView& v) {
+  if (kv_check(c, s, what)) return -1;
+  if (layer < 0 || layer >= c->n_layers) {
+    set_error("%s: layer %d of %d", what, layer, c->n_layers);
+    return -1;
+  }
+  if (n_rows < 0 || (n_rows && !row_start)) {
+    set_error("%s: %d rows, row_start %p", what, n_rows, (const void*)row_start);
+    return -1;
+  }
+  const int64_t head = (int64_t)(c->page_tokens / kKvBlock) * 2 * kv_tiles(c->head_dim) * kKvTile;
+  const int64_t head_scales = (int64_t)(c->page_tokens / kKvBlock) * 2;
+  v = KvView{};
+  v.codes = c->codes + layer * c->n_kv_heads * head;
+  v.scales = c->scales + layer * c->n_kv_heads * head_scales;
+  v.page_codes = c->n_layers * c->n_kv_heads * head;
+  v.page_scales = c->n_layers * c->n_kv_heads * head_scales;
+  v.n_kv_heads = c->n_kv_heads, v.D = c->head_dim, v.blocks = c->page_tokens / kKvBlock;
+  v.n_pages = c->n_pages, v.n_seqs = s->n_seqs, v.max_pages = s->max_pages;
+  v.table = s->table, v.len = s->len, v.refs = s->refs;
+  v.row_start = row_start, v.n_rows = n_rows;
+  v.fd_blocks = make_fastdiv((uint32_t)v.blocks);
+  return 0;
+}
+
+namespace {
+
+struct AppendArgs {
+  KvView v;
+  const float *k, *vv;
+  int k_stride, v_stride;
+  int groups;      // workgroups of a slot: four jobs (a head's k or v) each
+  FastDiv fd_groups;
+  int block_wgs;   // workgroups of the slots; those behind them rotate q rows
+  int rope;        // rotate
+  int k_vec, v_vec;  // float4 reads of k rows; of their partners by half a head too
+  int half_vec;
+  RopeRows r;      // the tables, and q
+};
+
+// x / s rounded to the nearest integer, ties to even, as the 64-bit quotient
+// rounds: x times the fp32 reciprocal is within 3e-5 of the quotient (|quotient|
+// below 128), which decides all but the values within 1e-4 of a tie; those
+// (and reciprocals that overflow) take the 64-bit division.
+__device__ __forceinline__ int quant(float x, float s, float inv) {
+  const float y = x * inv;
+  float r = __builtin_rintf(y);
+  if (!(__builtin_fabsf(y - r) < 0.4999f)) r = (float)__builtin_rint((double)x / (double)s);
+  return min(max((int)r, -127), 127);
+}
+// c * was / now likewise (was <= now: no clamp is needed).
+__device__ __forceinline__ int requant(int c, float was, float now, float ratio) {
+  const float y = (float)c * ratio;
+  float r = __builtin_rintf(y);
+  if (!(__builtin_fabsf(y - r) < 0.4999f))
+    r = (float)__builtin_rint((double)c * (double)was / (double)now);
+  return (int)r;
+}
+
+__device__ __forceinline__ float wave_amax(float x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x = vmax(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+// Eight elements of a row from d on, zeros from D on.
+__device__ __forceinline__ void load8(const float* row, int d, int D, int vec, float (&x)[8]) {
+  if (vec) {
+    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 a = d < D ? *(const float4*)(row + d) : z;
+    const float4 b = d + 4 < D ? *(const float4*)(row + d + 4) : z;
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = d + j < D ? row[d + j] : 0.0f;
+  }
+}
+
+// Elements d..d+7 of a k row, rotated to position pos.
+__device__ __forceinline__ void load_k8(const AppendArgs& a, const float* row, int d, int pos,
+                                        float (&x)[8]) {
+  load8(row, d, a.v.D, a.k_vec, x);
+  if (!a.rope || d >= a.r.rot) return;
+  const int half = a.r.rot / 2;
+  const bool known = pos < a.r.n_pos;
+  const size_t tab = (size_t)(known ? pos : 0) * half;
+  const float nan = __builtin_nanf("");
+  if (!a.r.qwen) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+      if (d + j < a.r.rot) {
+        const int i = (d + j) / 2;
+        rotate_pair(x[j], x[j + 1], known ? a.r.cos_t[tab + i] : nan,
+                    known ? a.r.sin_t[tab + i] : nan);
+      }
+    return;
+  }
+  // the partner of element e lies half a rotated part away
+  float y[8], c[8], s[8];
+  if (a.half_vec) {  // half is a multiple of 8: all eight on one side of it
+    const bool lo = d < half;
+    const int i = lo ? d : d - half;
+    load8(row, lo ? d + half : d - half, a.v.D, 1, y);
+    load8(a.r.cos_t + tab, i, half, 1, c);
+    load8(a.r.sin_t + tab, i, half, 1, s);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = d + j, i = e < half ? e : e - half;
+      const bool in = e < a.r.rot;
+      y[j] = in ? row[e < half ? e + half : e - half] : 0.0f;
+      c[j] = in ? a.r.cos_t[tab + i] : 1.0f;
+      s[j] = in ? a.r.sin_t[tab + i] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int e = d + j;
+    if (e >= a.r.rot) continue;
+    float x0 = e < half ? x[j] : y[j], x1 = e < half ? y[j] : x[j];
+    rotate_pair(x0, x1, known ? c[j] : nan, known ? s[j] : nan);
+    x[j] = e < half ? x0 : x1;
+  }
+}
+
+// A wave per touched block, kv head and k or v: the block's new rows in
+// registers in the order of its tiles (so each lane ends with 16 adjacent
+// bytes of every tile), their largest magnitude over the wave, the scale, the
+// codes.  Blocks with older rows read their tiles and put them back whole.
+//
+// HBM bounds prompts (4 bytes read and 1 written an element), latency single
+// tokens: row_start, len, table, rows and tiles are read one after the other.
+template <int DT>
+__global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
+  const KvView& v = a.v;
+  if ((int)blockIdx.x >= a.block_wgs) {  // q rows
+    const int item = (int)blockIdx.x - a.block_wgs;
+    const int row = (int)fdiv((uint32_t)item, a.r.fd_chunk);
+    const int s = kv_seq_of_row(v, row);
+    if (s >= v.n_seqs || row < v.row_start[0]) return;
+    int first, count;
+    kv_rows(v, s, first, count);
+    const int pos = kv_len(v, s) - count + (row - first);
+    if (pos >= 0) rope_row_items(a.r, row, item - row * a.r.chunks, pos);
+    return;
+  }
+  const int slot = (int)fdiv(blockIdx.x, a.fd_groups);
+  const int s = kv_seq_of_slot(v, slot);
+  const int job = ((int)blockIdx.x - slot * a.groups) * 4 + (int)(threadIdx.x >> 6);
+  if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
+  int row0, count;
+  kv_rows(v, s, row0, count);
+  const int len = kv_len(v, s);
+  const int start = len - count;  // position of row row0 (negative: rows dropped)
+  const int lo = max(start, 0);
+  const int blk = lo / kKvBlock + slot - kv_first_slot(v, s);
+  if (count == 0 || blk * kKvBlock >= len) return;
+  const int page = kv_page(v, s, blk);
+  if (page < 0 || v.refs[page] != 1) return;
+  const int head = job >> 1, is_v = job & 1;
+  const int b = blk - (int)fdiv((uint32_t)blk, v.fd_blocks) * v.blocks;
+  const int unit = (head * v.blocks + b) * 2 + is_v;
+  uint4* tiles = (uint4*)(v.codes + page * v.page_codes + (int64_t)unit * DT * kKvTile);
+  float* scale = v.scales + page * v.page_scales + unit;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int t0 = blk * kKvBlock;
+  const bool older = lo > t0;
+
+  uint4 old[DT];
+  float was = 0.0f;
+  if (older) {
+    was = *scale;
+#pragma unroll
+    for (int c = 0; c < DT; ++c) old[c] = tiles[c * 64 + lane];
+  } else {
+#pragma unroll
+    for (int c = 0; c < DT; ++c) old[c] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  // x[c][8 h + j]: the element whose code is byte 8 h + j of this lane's sixteen
+  float x[DT][16];
+  if (!is_v) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int pos = t0 + 16 * h + i;
+      const bool fresh = pos >= lo && pos < len;
+      const float* row = a.k + (int64_t)(row0 + (fresh ? pos : lo) - start) * a.k_stride +
+                         head * v.D;
+#pragma unroll
+      for (int c = 0; c < DT; ++c) {
+        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (fresh) load_k8(a, row, 32 * c + 8 * g, pos, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[c][8 * h + j] = y[j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int pos = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+      const bool fresh = pos >= lo && pos < len;
+      const float* row = a.vv + (int64_t)(row0 + (fresh ? pos : lo) - start) * a.v_stride +
+                         head * v.D;
+#pragma unroll
+      for (int c = 0; c < DT; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = 32 * c + 16 * h + i;
+          x[c][8 * h + j] = fresh && d < v.D ? row[d] : 0.0f;
+        }
+    }
+  }
+  float amax = 0.0f;
+#pragma unroll
+  for (int c = 0; c < DT; ++c)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = vmax(amax, __builtin_fabsf(x[c][j]));
+  amax = wave_amax(amax);
+
+  const float need = amax / 127.0f;
+  float now = older ? fmaxf(was, need) : need;
+  const bool bad = !(amax < INFINITY) || !(was < INFINITY);
+  if (bad) now = __builtin_nanf("");
+  const bool grown = older && now > was;  // false where bad
+  const float ratio = grown ? was / now : 1.0f;
+  const bool zero = bad || now == 0.0f;
+  const float inv = zero ? 0.0f : 1.0f / now;
+#pragma unroll
+  for (int c = 0; c < DT; ++c) {
+    uint32_t w[4] = {old[c].x, old[c].y, old[c].z, old[c].w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t out = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = 4 * q + e, h = n >> 3, j = n & 7;
+        const int t = is_v ? 16 * (j >> 2) + 4 * g + (j & 3) : 16 * h + i;
+        const bool fresh = t0 + t >= lo && t0 + t < len;
+        int code = (int)(int8_t)(w[q] >> (8 * e));
+        if (fresh)
+          code = zero ? 0 : quant(x[c][n], now, inv);
+        else if (grown)
+          code = requant(code, was, now, ratio);
+        out |= (uint32_t)(code & 0xFF) << (8 * e);
+      }
+      w[q] = out;
+    }
+    tiles[c * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (lane == 0) *scale = now;
+}
+
+struct FetchArgs {
+  KvView v;
+  float *k, *vv;
+  int k_stride, v_stride, k_vec;
+  int groups;
+  FastDiv fd_groups;
+};
+
+// A wave per block, kv head and k or v, as the append: 16 adjacent codes a lane
+// and tile.  HBM (the 4-byte values written) bounds it.
+template <int DT>
+__global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
+  const KvView& v = a.v;
+  const int slot = (int)fdiv(blockIdx.x, a.fd_groups);
+  const int s = kv_seq_of_slot(v, slot);
+  const int job = ((int)blockIdx.x - slot * a.groups) * 4 + (int)(threadIdx.x >> 6);
+  if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
+  int row0, count;
+  kv_rows(v, s, row0, count);
+  if (count == 0) return;
+  const int len = kv_len(v, s), start = len - count, lo = max(start, 0);
+  const int head = job >> 1, is_v = job & 1;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  float* dst = (is_v ? a.vv : a.k) + head * v.D;
+  const int stride = is_v ? a.v_stride : a.k_stride;
+  const int local = slot - kv_first_slot(v, s);
+  if (start < 0 && local == 0) {  // rows before position 0
+    for (int r = 0; r < min(-start, count); ++r)
+      for (int d = lane; d < v.D; d += 64) dst[(int64_t)(row0 + r) * stride + d] = 0.0f;
+  }
+  const int blk = lo / kKvBlock + local;
+  if (blk * kKvBlock >= len) return;
+  const int page = kv_page(v, s, blk), src = page < 0 ? 0 : page;
+  const int b = blk - (int)fdiv((uint32_t)blk, v.fd_blocks) * v.blocks;
+  const int unit = (head * v.blocks + b) * 2 + is_v;
+  const uint4* tiles = (const uint4*)(v.codes + src * v.page_codes + (int64_t)unit * DT * kKvTile);
+  const float scale = page < 0 ? __builtin_nanf("") : v.scales[src * v.page_scales + unit];
+  const int t0 = blk * kKvBlock;
+  uint4 tile[DT];
+#pragma unroll
+  for (int c = 0; c < DT; ++c) tile[c] = tiles[c * 64 + lane];
+#pragma unroll
+  for (int c = 0; c < DT; ++c) {
+    const uint32_t w[4] = {tile[c].x, tile[c].y, tile[c].z, tile[c].w};
+    float y[16];
+#pragma unroll
+    for (int n = 0; n < 16; ++n) y[n] = (float)(int)(int8_t)(w[n >> 2] >> (8 * (n & 3))) * scale;
+    if (!is_v) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int pos = t0 + 16 * h + i, d = 32 * c + 8 * g;
+        if (pos < lo || pos >= len) continue;
+        float* row = dst + (int64_t)(row0 + pos - start) * stride;
+        if (a.k_vec) {
+          if (d < v.D)
+            *(float4*)(row + d) = make_float4(y[8 * h], y[8 * h + 1], y[8 * h + 2], y[8 * h + 3]);
+          if (d + 4 < v.D)
+            *(float4*)(row + d + 4) =
+                make_float4(y[8 * h + 4], y[8 * h + 5], y[8 * h + 6], y[8 * h + 7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (d + j < v.D) row[d + j] = y[8 * h + j];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int pos = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+        if (pos < lo || pos >= len) continue;
+        float* row = dst + (int64_t)(row0 + pos - start) * stride;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (32 * c + 16 * h + i < v.D) row[32 * c + 16 * h + i] = y[8 * h + j];
+      }
+    }
+  }
+}
+
+// Pointer and row stride of rows of n heads; strides cover the rows.
+int check_rows(const char* what, const char* name, const void* p, int n_heads, int D, int stride) {
+  if (!p || ((uintptr_t)p & 3)) {
+    set_error("%s: %s is null or not aligned", what, name);
+    return -1;
+  }
+  if ((int64_t)n_heads * D > stride) {
+    set_error("%s: %s rows of %d heads of %d are %d floats apart", what, name, n_heads, D, stride);
+    return -1;
+  }
+  return 0;
+}
+
+bool quads(const void* p, int stride, int D) {
+  return (((uintptr_t)p | (uintptr_t)stride * 4 | (uintptr_t)D * 4) & 15) == 0;
+}
+
+template <int DT>
+void launch_append(const AppendArgs& a, unsigned wgs) {
+  hipLaunchKernelGGL(kv8_append_kernel<DT>, dim3(wgs), dim3(kKvThreads), 0, ctx().stream, a);
+}
+template <int DT>
+void launch_fetch(const FetchArgs& a, unsigned wgs) {
+  hipLaunchKernelGGL(kv8_fetch_kernel<DT>, dim3(wgs), dim3(kKvThreads), 0, ctx().stream, a);
+}
+
+}  // namespace
+}  // namespace plh
+
+using namespace plh;
+
+#define PLH_KV_TILES(dt, fn, ...)                    \
+  switch (dt) {                                      \
+    case 1: fn<1>(__VA_ARGS__); break;               \
+    case 2: fn<2>(__VA_ARGS__); break;               \
+    case 3: fn<3>(__VA_ARGS__); break;               \
+    case 4: fn<4>(__VA_ARGS__); break;               \
+    case 5: fn<5>(__VA_ARGS__); break;               \
+    case 6: fn<6>(__VA_ARGS__); break;               \
+    case 7: fn<7>(__VA_ARGS__); break;               \
+    default: fn<8>(__VA_ARGS__); break;              \
+  }
+
+extern "C" {
+
+size_t plh_kv8_code_bytes(const plh_kv8_cache* c) {
+  if (!c || c->n_layers < 1 || c->n_kv_heads < 1 || c->head_dim < 2 || c->head_dim > 256 ||
+      (c->head_dim & 1) || c->n_pages < 1 || c->page_tokens < kKvBlock ||
+      c->page_tokens % kKvBlock)
+    return 0;
+  const int64_t tiles = (int64_t)(c->page_tokens / kKvBlock) * 2 * kv_tiles(c->head_dim);
+  const int64_t heads = (int64_t)c->n_layers * c->n_kv_heads;
+  if (heads > INT_MAX || tiles > INT_MAX / kKvTile || heads * tiles > INT_MAX / kKvTile) return 0;
+  return (size_t)(heads * tiles) * kKvTile * (size_t)c->n_pages;
+}
+
+size_t plh_kv8_scale_bytes(const plh_kv8_cache* c) {
+  const size_t codes = plh_kv8_code_bytes(c);
+  return codes ? codes / ((size_t)kv_tiles(c->head_dim) * kKvTile) * sizeof(float) : 0;
+}
+
+int plh_kv8_append(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int layer, int n_rows,
+                   const int32_t* row_start, const plh_rope* rope, const float* q, int n_heads,
+                   int q_stride, float* q_out, int q_out_stride, const float* k, int k_stride,
+                   const float* v, int v_stride) {
+  const char* what = "plh_kv8_append";
+  AppendArgs a{};
+  if (kv_view(cache, seqs, layer, n_rows, row_start, what, a.v)) return -1;
+  const int D = cache->head_dim, H = cache->n_kv_heads;
+  if (n_heads < 0 || (n_heads && !rope)) {
+    set_error("%s: %d q heads are rotated by tables only", what, n_heads);
+    return -1;
+  }
+  if (rope && check_rope(rope, D, what)) return -1;
+  if (n_rows && (check_rows(what, "k", k, H, D, k_stride) ||
+                 check_rows(what, "v", v, H, D, v_stride) ||
+                 (n_heads && (check_rows(what, "q", q, n_heads, D, q_stride) ||
+                              check_rows(what, "q_out", q_out, n_heads, D, q_out_stride)))))
+    return -1;
+  if ((int64_t)n_heads * D > INT_MAX / 2) {
+    set_error("%s: %d q heads are too many", what, n_heads);
+    return -1;
+  }
+  a.k = k, a.vv = v, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.groups = (2 * H + 3) / 4;
+  a.fd_groups = make_fastdiv((uint32_t)a.groups);
+  a.k_vec = quads(k, k_stride, D);
+  a.rope = rope != nullptr;
+  int64_t wgs = kv_slots(n_rows, seqs->n_seqs) * a.groups;
+  if (rope) {
+    a.r = rope_rows_args(rope, D, q, n_heads, q_stride, q_out, q_out_stride, nullptr, 0, 0,
+                         nullptr, 0);
+    a.half_vec = a.k_vec && rope->rot_dim % 16 == 0 &&
+                 (((uintptr_t)rope->cos_tab | (uintptr_t)rope->sin_tab) & 15) == 0;
+  }
+  a.block_wgs = (int)(wgs < INT_MAX ? wgs : INT_MAX);
+  if (n_heads) wgs += (int64_t)n_rows * a.r.chunks;
+  if (wgs > kMaxWorkgroups) {
+    set_error("%s: %d rows of %d sequences are too many for one call", what, n_rows, seqs->n_seqs);
+    return -1;
+  }
+  if (kv_ready(what)) return -1;
+  if (n_rows == 0) return 0;
+  PLH_KV_TILES(kv_tiles(D), launch_append, a, (unsigned)wgs);
+  return check_hip(hipGetLastError(), "kv8_append_kernel");
+}
+
+int plh_kv8_fetch(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int layer, int n_rows,
+                  const int32_t* row_start, float* k, int k_stride, float* v, int v_stride) {
+  const char* what = "plh_kv8_fetch";
+  FetchArgs a{};
+  if (kv_view(cache, seqs, layer, n_rows, row_start, what, a.v)) return -1;
+  const int D = cache->head_dim, H = cache->n_kv_heads;
+  if (n_rows && (check_rows(what, "k", k, H, D, k_stride) ||
+                 check_rows(what, "v", v, H, D, v_stride)))
+    return -1;
+  a.k = k, a.vv = v, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.k_vec = quads(k, k_stride, D);
+  a.groups = (2 * H + 3) / 4;
+  a.fd_groups = make_fastdiv((uint32_t)a.groups);
+  const int64_t wgs = kv_slots(n_rows, seqs->n_seqs) * a.groups;
+  if (wgs > kMaxWorkgroups) {
+    set_error("%s: %d rows of %d sequences are too many for one call", what, n_rows, seqs->n_seqs);
+    return -1;
+  }
+  if (kv_ready(what)) return -1;
+  if (n_rows == 0) return 0;
+  PLH_KV_TILES(kv_tiles(D), launch_fetch, a, (unsigned)wgs);
+  return check_hip(hipGetLastError(), "kv8_fetch_kernel");
+}
+
+}  // extern "C"
