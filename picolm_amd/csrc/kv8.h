@@ -63,27 +63,52 @@ __device__ __forceinline__ int kv_page(const KvView& v, int s, int block) {
 // i-th touched block.  Slots without a block do nothing.
 inline int64_t kv_slots(int n_rows, int n_seqs) { return n_rows / kKvBlock + 2ll * n_seqs; }
 
-// Sequence of a slot (n_seqs: none); every thread of the workgroup calls it.
-__device__ __forceinline__ int kv_seq_of_slot(const KvView& v, int slot) {
-  int s = 0;
-  for (int at = 0; at < v.n_seqs; at += kKvThreads) {
-    const int i = at + (int)threadIdx.x;
-    s += __syncthreads_count(
-        i < v.n_seqs && min(max(v.row_start[i + 1], 0), v.n_rows) / kKvBlock + 2 * (i + 1) <= slot);
+// What a wave knows of the first 64 sequences, a lane each: loaded together, so
+// that finding a row's or a slot's sequence costs one memory latency.
+struct KvLanes {
+  int start, next, len;  // row_start[lane], row_start[lane + 1], tokens
+};
+__device__ __forceinline__ KvLanes kv_lanes(const KvView& v) {
+  const int lane = (int)threadIdx.x & 63;
+  KvLanes l{0, 0, 0};
+  if (lane < v.n_seqs) {
+    l.start = v.row_start[lane];
+    l.next = v.row_start[lane + 1];
+    l.len = v.len[lane];
+  }
+  return l;
+}
+// The number of sequences i for which before(i, row_start[i + 1]) holds: with
+// row_start rising, the first sequence for which it does not (n_seqs: none).
+template <class F>
+__device__ __forceinline__ int kv_find(const KvView& v, const KvLanes& l, F before) {
+  const int lane = (int)threadIdx.x & 63;
+  int s = __popcll(__ballot(lane < v.n_seqs && before(lane, l.next)));
+  for (int at = 64; at < v.n_seqs; at += 64) {
+    const int i = at + lane;
+    s += __popcll(__ballot(i < v.n_seqs && before(i, v.row_start[min(i, v.n_seqs - 1) + 1])));
   }
   return s;
 }
-__device__ __forceinline__ int kv_first_slot(const KvView& v, int s) {
-  return min(max(v.row_start[s], 0), v.n_rows) / kKvBlock + 2 * s;
-}
-// Sequence of a row, likewise.
-__device__ __forceinline__ int kv_seq_of_row(const KvView& v, int row) {
-  int s = 0;
-  for (int at = 0; at < v.n_seqs; at += kKvThreads) {
-    const int i = at + (int)threadIdx.x;
-    s += __syncthreads_count(i < v.n_seqs && v.row_start[i + 1] <= row);
+// Rows (as kv_rows) and tokens of sequence s, from the lanes where they hold it.
+struct KvSeq {
+  int row0, count, len;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvView& v, const KvLanes& l, int s) {
+  int a, b, n;
+  if (s < 64) {
+    a = __builtin_amdgcn_readlane(l.start, s);
+    b = __builtin_amdgcn_readlane(l.next, s);
+    n = __builtin_amdgcn_readlane(l.len, s);
+  } else {
+    a = v.row_start[s], b = v.row_start[s + 1], n = v.len[s];
   }
-  return s;
+  a = min(max(a, 0), v.n_rows);
+  b = min(max(b, a), v.n_rows);
+  return KvSeq{a, b - a, min(max(n, 0), v.max_pages * v.blocks * kKvBlock)};
+}
+__device__ __forceinline__ int kv_slot_key(const KvView& v, int i, int start) {
+  return min(max(start, 0), v.n_rows) / kKvBlock + 2 * i;
 }
 
 }  // namespace plh

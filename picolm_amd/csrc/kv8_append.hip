@@ -76,11 +76,14 @@ struct AppendArgs {
   int groups;      // workgroups of a slot: four jobs (a head's k or v) each
   FastDiv fd_groups;
   int block_wgs;   // workgroups of the slots; those behind them rotate q rows
+  int q_rows;      // rows of such a workgroup (1..kQRows)
   int rope;        // rotate
   int k_vec, v_vec;  // float4 reads of k rows; of their partners by half a head too
   int half_vec;
   RopeRows r;      // the tables, and q
 };
+
+constexpr int kQRows = 4;
 
 // x / s rounded to the nearest integer, ties to even, as the 64-bit quotient
 // rounds: x times the fp32 reciprocal is within 3e-5 of the quotient (|quotient|
@@ -168,68 +171,135 @@ __device__ __forceinline__ void load_k8(const AppendArgs& a, const float* row, i
   }
 }
 
-// A wave per touched block, kv head and k or v: the block's new rows in
-// registers in the order of its tiles (so each lane ends with 16 adjacent
-// bytes of every tile), their largest magnitude over the wave, the scale, the
-// codes.  Blocks with older rows read their tiles and put them back whole.
-//
-// HBM bounds prompts (4 bytes read and 1 written an element), latency single
-// tokens: row_start, len, table, rows and tiles are read one after the other.
-template <int DT>
-__global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
-  const KvView& v = a.v;
-  if ((int)blockIdx.x >= a.block_wgs) {  // q rows
-    const int item = (int)blockIdx.x - a.block_wgs;
-    const int row = (int)fdiv((uint32_t)item, a.r.fd_chunk);
-    const int s = kv_seq_of_row(v, row);
-    if (s >= v.n_seqs || row < v.row_start[0]) return;
-    int first, count;
-    kv_rows(v, s, first, count);
-    const int pos = kv_len(v, s) - count + (row - first);
-    if (pos >= 0) rope_row_items(a.r, row, item - row * a.r.chunks, pos);
-    return;
-  }
-  const int slot = (int)fdiv(blockIdx.x, a.fd_groups);
-  const int s = kv_seq_of_slot(v, slot);
-  const int job = ((int)blockIdx.x - slot * a.groups) * 4 + (int)(threadIdx.x >> 6);
-  if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
-  int row0, count;
-  kv_rows(v, s, row0, count);
-  const int len = kv_len(v, s);
-  const int start = len - count;  // position of row row0 (negative: rows dropped)
-  const int lo = max(start, 0);
-  const int blk = lo / kKvBlock + slot - kv_first_slot(v, s);
-  if (count == 0 || blk * kKvBlock >= len) return;
-  const int page = kv_page(v, s, blk);
-  if (page < 0 || v.refs[page] != 1) return;
-  const int head = job >> 1, is_v = job & 1;
-  const int b = blk - (int)fdiv((uint32_t)blk, v.fd_blocks) * v.blocks;
-  const int unit = (head * v.blocks + b) * 2 + is_v;
-  uint4* tiles = (uint4*)(v.codes + page * v.page_codes + (int64_t)unit * DT * kKvTile);
-  float* scale = v.scales + page * v.page_scales + unit;
-  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-  const int t0 = blk * kKvBlock;
-  const bool older = lo > t0;
+// A block's place and its new rows.
+struct Place {
+  int row0, start;  // first row of the sequence's, and its position
+  int t0, lo, len;  // the block's first token; new rows are positions lo..len-1
+  int head, is_v;
+};
 
-  uint4 old[DT];
-  float was = 0.0f;
-  if (older) {
-    was = *scale;
-#pragma unroll
-    for (int c = 0; c < DT; ++c) old[c] = tiles[c * 64 + lane];
-  } else {
-#pragma unroll
-    for (int c = 0; c < DT; ++c) old[c] = make_uint4(0u, 0u, 0u, 0u);
+// The block's scale, given the largest magnitude of its new rows.
+struct Scale {
+  float was, now, ratio, inv;
+  bool grown, zero;
+  __device__ __forceinline__ Scale(float amax, float was_, bool older) : was(was_) {
+    const float need = amax / 127.0f;
+    now = older ? fmaxf(was, need) : need;
+    const bool bad = !(amax < INFINITY) || !(was < INFINITY);
+    if (bad) now = __builtin_nanf("");
+    grown = older && now > was;  // false where bad
+    ratio = grown ? was / now : 1.0f;
+    zero = bad || now == 0.0f;
+    inv = zero ? 0.0f : 1.0f / now;
   }
+  __device__ __forceinline__ int code(float x) const { return zero ? 0 : quant(x, now, inv); }
+};
+
+// Sixteen codes of a lane rounded again.
+__device__ __forceinline__ uint4 requant16(uint4 old, const Scale& s) {
+  uint32_t w[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      out |= (uint32_t)(requant((int)(int8_t)(w[q] >> (8 * e)), s.was, s.now, s.ratio) & 0xFF)
+             << (8 * e);
+    w[q] = out;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One new row in a block (a single token): two elements a lane at a time, the pairs
+// that rotate together, and single bytes stored.  The block's tiles are only
+// touched where its scale grows, or cleared where the row begins it.
+template <int DT>
+__device__ __forceinline__ void append_row(const AppendArgs& a, const Place& p, uint4* tiles,
+                                           float* scale, bool may_store) {
+  constexpr int kPairs = (16 * DT + 63) / 64;  // of a lane
+  const int lane = threadIdx.x & 63, D = a.v.D;
+  const int pos = max(p.t0, p.lo), t = pos - p.t0;
+  const bool older = p.lo > p.t0;
+  const float* row = (p.is_v ? a.vv + (int64_t)(p.row0 + pos - p.start) * a.v_stride
+                             : a.k + (int64_t)(p.row0 + pos - p.start) * a.k_stride) +
+                     p.head * D;
+  const float was = older ? *scale : 0.0f;
+  const bool turn = !p.is_v && a.rope;
+  const int rot = turn ? a.r.rot : 0, half = rot / 2;
+  const bool known = pos < a.r.n_pos;
+  const int64_t tab = (int64_t)(known ? pos : 0) * half;
+  float x[kPairs][2];
+  int d[kPairs][2];
+  float amax = 0.0f;
+#pragma unroll
+  for (int n = 0; n < kPairs; ++n) {
+    const int i = lane + 64 * n;
+    const bool in = i < D / 2, rotates = i < half;
+    d[n][0] = rotates && a.r.qwen ? i : 2 * i;
+    d[n][1] = rotates && a.r.qwen ? i + half : 2 * i + 1;
+    x[n][0] = in ? row[d[n][0]] : 0.0f;
+    x[n][1] = in ? row[d[n][1]] : 0.0f;
+    if (rotates) {
+      const float nan = __builtin_nanf("");
+      const float c = a.r.cos_t[tab + i], s = a.r.sin_t[tab + i];
+      rotate_pair(x[n][0], x[n][1], known ? c : nan, known ? s : nan);
+    }
+    amax = vmax(amax, vmax(__builtin_fabsf(x[n][0]), __builtin_fabsf(x[n][1])));
+  }
+  const Scale s(wave_amax(amax), was, older);
+  if (!may_store) return;
+  if (s.grown || !older) {
+#pragma unroll 1
+    for (int c = 0; c < DT; ++c)
+      tiles[c * 64 + lane] =
+          older ? requant16(tiles[c * 64 + lane], s) : make_uint4(0u, 0u, 0u, 0u);
+    // the bytes below lie in other lanes' sixteen
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+  }
+  int8_t* bytes = (int8_t*)tiles;
+#pragma unroll
+  for (int n = 0; n < kPairs; ++n)
+    if (lane + 64 * n < D / 2)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int k = d[n][e], in = k & 31;
+        const int at = p.is_v
+                           ? 256 * ((t & 15) >> 2) + 16 * (in & 15) + 8 * (in >> 4) +
+                                 4 * (t >> 4) + (t & 3)
+                           : 256 * (in >> 3) + 16 * (t & 15) + 8 * (t >> 4) + (in & 7);
+        bytes[(k >> 5) * kKvTile + at] = (int8_t)s.code(x[n][e]);
+      }
+  // elements behind D of the last tile
+  for (int k = D + lane; k < 32 * DT; k += 64) {
+    const int in = k & 31;
+    const int at = p.is_v ? 256 * ((t & 15) >> 2) + 16 * (in & 15) + 8 * (in >> 4) + 4 * (t >> 4) +
+                                (t & 3)
+                          : 256 * (in >> 3) + 16 * (t & 15) + 8 * (t >> 4) + (in & 7);
+    bytes[(k >> 5) * kKvTile + at] = 0;
+  }
+  if (lane == 0) *scale = s.now;
+}
+
+// Several new rows: in registers in the order of the tiles (so each lane ends
+// with 16 adjacent bytes of every tile).  Blocks with older rows read their tiles
+// and put them back whole.
+template <int DT>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p, const int32_t* entry,
+                                            int b) {
+  const KvView& v = a.v;
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const bool older = p.lo > p.t0;
+  const int page = *entry;
   // x[c][8 h + j]: the element whose code is byte 8 h + j of this lane's sixteen
   float x[DT][16];
-  if (!is_v) {
+  if (!p.is_v) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int pos = t0 + 16 * h + i;
-      const bool fresh = pos >= lo && pos < len;
-      const float* row = a.k + (int64_t)(row0 + (fresh ? pos : lo) - start) * a.k_stride +
-                         head * v.D;
+      const int pos = p.t0 + 16 * h + i;
+      const bool fresh = pos >= p.lo && pos < p.len;
+      const float* row = a.k + (int64_t)(p.row0 + (fresh ? pos : p.lo) - p.start) * a.k_stride +
+                         p.head * v.D;
 #pragma unroll
       for (int c = 0; c < DT; ++c) {
         float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -241,10 +311,10 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int pos = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-      const bool fresh = pos >= lo && pos < len;
-      const float* row = a.vv + (int64_t)(row0 + (fresh ? pos : lo) - start) * a.v_stride +
-                         head * v.D;
+      const int pos = p.t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+      const bool fresh = pos >= p.lo && pos < p.len;
+      const float* row = a.vv + (int64_t)(p.row0 + (fresh ? pos : p.lo) - p.start) * a.v_stride +
+                         p.head * v.D;
 #pragma unroll
       for (int c = 0; c < DT; ++c)
 #pragma unroll
@@ -254,44 +324,106 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
         }
     }
   }
+  if (page < 0 || page >= v.n_pages || v.refs[page] != 1) return;
+  const int unit = (p.head * v.blocks + b) * 2 + p.is_v;
+  uint4* tiles = (uint4*)(v.codes + page * v.page_codes + (int64_t)unit * DT * kKvTile);
+  float* scale = v.scales + page * v.page_scales + unit;
+  uint4 old[DT];
+  float was = 0.0f;
+  if (older) {
+    was = *scale;
+#pragma unroll
+    for (int c = 0; c < DT; ++c) old[c] = tiles[c * 64 + lane];
+  } else {
+#pragma unroll
+    for (int c = 0; c < DT; ++c) old[c] = make_uint4(0u, 0u, 0u, 0u);
+  }
   float amax = 0.0f;
 #pragma unroll
   for (int c = 0; c < DT; ++c)
 #pragma unroll
     for (int j = 0; j < 16; ++j) amax = vmax(amax, __builtin_fabsf(x[c][j]));
-  amax = wave_amax(amax);
-
-  const float need = amax / 127.0f;
-  float now = older ? fmaxf(was, need) : need;
-  const bool bad = !(amax < INFINITY) || !(was < INFINITY);
-  if (bad) now = __builtin_nanf("");
-  const bool grown = older && now > was;  // false where bad
-  const float ratio = grown ? was / now : 1.0f;
-  const bool zero = bad || now == 0.0f;
-  const float inv = zero ? 0.0f : 1.0f / now;
+  const Scale s(wave_amax(amax), was, older);
 #pragma unroll
   for (int c = 0; c < DT; ++c) {
-    uint32_t w[4] = {old[c].x, old[c].y, old[c].z, old[c].w};
+    const uint4 kept = s.grown ? requant16(old[c], s) : old[c];
+    uint32_t w[4] = {kept.x, kept.y, kept.z, kept.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      uint32_t out = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int n = 4 * q + e, h = n >> 3, j = n & 7;
-        const int t = is_v ? 16 * (j >> 2) + 4 * g + (j & 3) : 16 * h + i;
-        const bool fresh = t0 + t >= lo && t0 + t < len;
-        int code = (int)(int8_t)(w[q] >> (8 * e));
-        if (fresh)
-          code = zero ? 0 : quant(x[c][n], now, inv);
-        else if (grown)
-          code = requant(code, was, now, ratio);
-        out |= (uint32_t)(code & 0xFF) << (8 * e);
+        const int t = p.is_v ? 16 * (j >> 2) + 4 * g + (j & 3) : 16 * h + i;
+        const bool fresh = p.t0 + t >= p.lo && p.t0 + t < p.len;
+        const uint32_t code = (uint32_t)(s.code(x[c][n]) & 0xFF) << (8 * e);
+        w[q] = fresh ? (w[q] & ~(0xFFu << (8 * e))) | code : w[q];
       }
-      w[q] = out;
     }
     tiles[c * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (lane == 0) *scale = now;
+  if (lane == 0) *scale = s.now;
+}
+
+// A wave per touched block, kv head and k or v (their rows' largest magnitude, the
+// scale, the codes), and behind them workgroups that rotate q rows.
+//
+// HBM bounds prompts (4 bytes read and 1 written an element); single tokens are
+// three memory latencies: row_start with len, the row with the page number, the
+// page's count and scale.
+template <int DT>
+__global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
+  const KvView& v = a.v;
+  if ((int)blockIdx.x >= a.block_wgs) {
+    const int wg = (int)blockIdx.x - a.block_wgs;
+    const int group = (int)fdiv((uint32_t)wg, a.r.fd_chunk);
+    const int item = (wg - group * a.r.chunks) * kRopeThreads + (int)threadIdx.x;
+    const KvLanes lanes = kv_lanes(v);
+    const int first = v.row_start[0];
+    RopeItem it[kQRows];
+#pragma unroll
+    for (int n = 0; n < kQRows; ++n) {
+      const int64_t row = (int64_t)group * a.q_rows + n;
+      if (n < a.q_rows && row < v.n_rows && item < a.r.per_row) it[n] = rope_load(a.r, row, item);
+    }
+#pragma unroll
+    for (int n = 0; n < kQRows; ++n) {
+      const int64_t row = (int64_t)group * a.q_rows + n;
+      if (n >= a.q_rows || row >= v.n_rows) continue;
+      const int s = kv_find(v, lanes, [&](int, int next) { return next <= row; });
+      if (s >= v.n_seqs || row < first) continue;
+      const KvSeq q = kv_seq(v, lanes, s);
+      const int pos = q.len - q.count + (int)row - q.row0;
+      if (pos >= 0 && item < a.r.per_row) rope_store(a.r, it[n], pos);
+    }
+    return;
+  }
+  const int slot = (int)fdiv(blockIdx.x, a.fd_groups);
+  const int job = ((int)blockIdx.x - slot * a.groups) * 4 +
+                  __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const KvLanes lanes = kv_lanes(v);
+  const int s =
+      kv_find(v, lanes, [&](int i, int next) { return kv_slot_key(v, i + 1, next) <= slot; });
+  if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
+  const KvSeq q = kv_seq(v, lanes, s);
+  Place p;
+  p.row0 = q.row0, p.len = q.len;
+  p.start = q.len - q.count;  // negative: rows before position 0 are dropped
+  p.lo = max(p.start, 0);
+  const int blk = p.lo / kKvBlock + slot - kv_slot_key(v, s, q.row0);
+  p.t0 = blk * kKvBlock;
+  if (q.count == 0 || p.t0 >= q.len) return;
+  p.head = job >> 1, p.is_v = job & 1;
+  const int e = (int)fdiv((uint32_t)blk, v.fd_blocks), b = blk - e * v.blocks;
+  const int32_t* entry = v.table + (size_t)s * v.max_pages + e;
+  if (min(p.len, p.t0 + kKvBlock) - max(p.lo, p.t0) > 1) {
+    append_rows<DT>(a, p, entry, b);
+    return;
+  }
+  const int page = *entry;
+  const bool ok = page >= 0 && page < v.n_pages;
+  const int at = ok ? page : 0, unit = (p.head * v.blocks + b) * 2 + p.is_v;
+  append_row<DT>(a, p, (uint4*)(v.codes + at * v.page_codes + (int64_t)unit * DT * kKvTile),
+                 v.scales + at * v.page_scales + unit, ok && v.refs[at] == 1);
 }
 
 struct FetchArgs {
@@ -308,18 +440,21 @@ template <int DT>
 __global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
   const KvView& v = a.v;
   const int slot = (int)fdiv(blockIdx.x, a.fd_groups);
-  const int s = kv_seq_of_slot(v, slot);
-  const int job = ((int)blockIdx.x - slot * a.groups) * 4 + (int)(threadIdx.x >> 6);
+  const int job = ((int)blockIdx.x - slot * a.groups) * 4 +
+                  __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const KvLanes lanes = kv_lanes(v);
+  const int s =
+      kv_find(v, lanes, [&](int i, int next) { return kv_slot_key(v, i + 1, next) <= slot; });
   if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
-  int row0, count;
-  kv_rows(v, s, row0, count);
+  const KvSeq q = kv_seq(v, lanes, s);
+  const int row0 = q.row0, count = q.count, len = q.len;
   if (count == 0) return;
-  const int len = kv_len(v, s), start = len - count, lo = max(start, 0);
+  const int start = len - count, lo = max(start, 0);
   const int head = job >> 1, is_v = job & 1;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   float* dst = (is_v ? a.vv : a.k) + head * v.D;
   const int stride = is_v ? a.v_stride : a.k_stride;
-  const int local = slot - kv_first_slot(v, s);
+  const int local = slot - kv_slot_key(v, s, row0);
   if (start < 0 && local == 0) {  // rows before position 0
     for (int r = 0; r < min(-start, count); ++r)
       for (int d = lane; d < v.D; d += 64) dst[(int64_t)(row0 + r) * stride + d] = 0.0f;
@@ -469,7 +604,10 @@ int plh_kv8_append(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int lay
                  (((uintptr_t)rope->cos_tab | (uintptr_t)rope->sin_tab) & 15) == 0;
   }
   a.block_wgs = (int)(wgs < INT_MAX ? wgs : INT_MAX);
-  if (n_heads) wgs += (int64_t)n_rows * a.r.chunks;
+  // Prompts: several rows' loads in flight a workgroup; while there are few rows,
+  // each has its own.
+  a.q_rows = n_rows >= 16 * ctx().num_cus ? kQRows : 1;
+  if (n_heads) wgs += (int64_t)((n_rows + a.q_rows - 1) / a.q_rows) * a.r.chunks;
   if (wgs > kMaxWorkgroups) {
     set_error("%s: %d rows of %d sequences are too many for one call", what, n_rows, seqs->n_seqs);
     return -1;

@@ -121,9 +121,14 @@ __global__ __launch_bounds__(256) void rope_tables_kernel(TableArgs a) {
   }
 }
 
+// A thread per item; the row's position arrives while its elements do.  HBM
+// bounds it: every element is read and written once.
 __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeRows a, const int32_t* pos) {
   const int row = (int)fdiv(blockIdx.x, a.fd_chunk);
-  rope_row_items(a, row, (int)blockIdx.x - row * a.chunks, pos[row]);
+  const int item = ((int)blockIdx.x - row * a.chunks) * kRopeThreads + (int)threadIdx.x;
+  if (item >= a.per_row) return;
+  const int p = pos[row];
+  rope_store(a, rope_load(a, row, item), p);
 }
 
 }  // namespace

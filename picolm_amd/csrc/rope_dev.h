@@ -40,51 +40,70 @@ __device__ __forceinline__ void rotate_pair(float& x0, float& x1, float c, float
   x1 = (float)__builtin_fma(a, sd, b * cd);
 }
 
-// Chunk `chunk` of row `row`'s items, one per thread.  Positions outside the
-// tables rotate by NaN.
-__device__ __forceinline__ void rope_row_items(const RopeRows& a, int row, int chunk, int pos) {
-  const int item = chunk * kRopeThreads + (int)threadIdx.x;
-  if (item >= a.per_row) return;
+// One item of a row: loaded before its position is known, then turned and
+// stored.  Positions outside the tables rotate by NaN.
+struct RopeItem {
+  float* y;
+  int i;       // number in its head
+  float4 x0, x1;
+};
+__device__ __forceinline__ RopeItem rope_load(const RopeRows& a, int64_t row, int item) {
+  RopeItem it;
   int head = (int)fdiv((uint32_t)item, a.fd_head);
-  const int i = item - head * a.per_head;
+  it.i = item - head * a.per_head;
   const bool is_q = head < a.n_heads;
   head -= is_q ? 0 : a.n_heads;
-  const float* x = (is_q ? a.q + (size_t)row * a.q_stride : a.k + (size_t)row * a.k_stride) +
-                   (size_t)head * a.D;
-  float* y = (is_q ? a.q_out + (size_t)row * a.q_out_stride
-                   : a.k_out + (size_t)row * a.k_out_stride) +
-             (size_t)head * a.D;
-  const bool known = pos >= 0 && pos < a.n_pos;
-  const size_t tab = (size_t)(known ? pos : 0) * (a.rot / 2);
-  const float nan = __builtin_nanf("");
+  const float* x = (is_q ? a.q + row * a.q_stride : a.k + row * a.k_stride) + (int64_t)head * a.D;
+  it.y = (is_q ? a.q_out + row * a.q_out_stride : a.k_out + row * a.k_out_stride) +
+         (int64_t)head * a.D;
+  it.x0 = it.x1 = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int i = it.i;
   if (i >= a.pairs) {  // behind the rotated part
     const int d = a.rot + (i - a.pairs) * (a.vec ? 4 : 1);
     if (a.vec)
-      *(float4*)(y + d) = *(const float4*)(x + d);
+      it.x0 = *(const float4*)(x + d);
     else
-      y[d] = x[d];
+      it.x0.x = x[d];
   } else if (!a.vec) {
-    const int d0 = a.qwen ? i : 2 * i, d1 = a.qwen ? i + a.rot / 2 : 2 * i + 1;
-    float x0 = x[d0], x1 = x[d1];
-    rotate_pair(x0, x1, known ? a.cos_t[tab + i] : nan, known ? a.sin_t[tab + i] : nan);
-    y[d0] = x0, y[d1] = x1;
+    it.x0.x = x[a.qwen ? i : 2 * i];
+    it.x1.x = x[a.qwen ? i + a.rot / 2 : 2 * i + 1];
   } else if (a.qwen) {
-    const int d0 = 4 * i, d1 = 4 * i + a.rot / 2;
-    float4 x0 = *(const float4*)(x + d0), x1 = *(const float4*)(x + d1);
-    float4 c = *(const float4*)(a.cos_t + tab + d0), s = *(const float4*)(a.sin_t + tab + d0);
-    if (!known) c = s = make_float4(nan, nan, nan, nan);
-    rotate_pair(x0.x, x1.x, c.x, s.x);
-    rotate_pair(x0.y, x1.y, c.y, s.y);
-    rotate_pair(x0.z, x1.z, c.z, s.z);
-    rotate_pair(x0.w, x1.w, c.w, s.w);
-    *(float4*)(y + d0) = x0, *(float4*)(y + d1) = x1;
+    it.x0 = *(const float4*)(x + 4 * i), it.x1 = *(const float4*)(x + 4 * i + a.rot / 2);
   } else {
-    float4 x0 = *(const float4*)(x + 4 * i);
+    it.x0 = *(const float4*)(x + 4 * i);
+  }
+  return it;
+}
+__device__ __forceinline__ void rope_store(const RopeRows& a, RopeItem it, int pos) {
+  const int i = it.i;
+  float* y = it.y;
+  const bool known = pos >= 0 && pos < a.n_pos;
+  const int64_t tab = (int64_t)(known ? pos : 0) * (a.rot / 2);
+  const float nan = __builtin_nanf("");
+  if (i >= a.pairs) {
+    const int d = a.rot + (i - a.pairs) * (a.vec ? 4 : 1);
+    if (a.vec)
+      *(float4*)(y + d) = it.x0;
+    else
+      y[d] = it.x0.x;
+  } else if (!a.vec) {
+    rotate_pair(it.x0.x, it.x1.x, known ? a.cos_t[tab + i] : nan, known ? a.sin_t[tab + i] : nan);
+    y[a.qwen ? i : 2 * i] = it.x0.x;
+    y[a.qwen ? i + a.rot / 2 : 2 * i + 1] = it.x1.x;
+  } else if (a.qwen) {
+    float4 c = *(const float4*)(a.cos_t + tab + 4 * i), s = *(const float4*)(a.sin_t + tab + 4 * i);
+    if (!known) c = s = make_float4(nan, nan, nan, nan);
+    rotate_pair(it.x0.x, it.x1.x, c.x, s.x);
+    rotate_pair(it.x0.y, it.x1.y, c.y, s.y);
+    rotate_pair(it.x0.z, it.x1.z, c.z, s.z);
+    rotate_pair(it.x0.w, it.x1.w, c.w, s.w);
+    *(float4*)(y + 4 * i) = it.x0, *(float4*)(y + 4 * i + a.rot / 2) = it.x1;
+  } else {
     float2 c = *(const float2*)(a.cos_t + tab + 2 * i), s = *(const float2*)(a.sin_t + tab + 2 * i);
     if (!known) c = s = make_float2(nan, nan);
-    rotate_pair(x0.x, x0.y, c.x, s.x);
-    rotate_pair(x0.z, x0.w, c.y, s.y);
-    *(float4*)(y + 4 * i) = x0;
+    rotate_pair(it.x0.x, it.x0.y, c.x, s.x);
+    rotate_pair(it.x0.z, it.x0.w, c.y, s.y);
+    *(float4*)(y + 4 * i) = it.x0;
   }
 }
 
