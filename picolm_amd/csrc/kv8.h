@@ -57,12 +57,6 @@ __device__ __forceinline__ int kv_page(const KvView& v, int s, int block) {
   return p >= 0 && p < v.n_pages ? p : -1;
 }
 
-// Slots.  The blocks that a batch's rows touch are numbered without a scan:
-// sequence s has the slots from row_start[s]/32 + 2 s on, at least as many as
-// its m rows can touch ((m + 30)/32 + 1 rounded down), and slot i of them is its
-// i-th touched block.  Slots without a block do nothing.
-inline int64_t kv_slots(int n_rows, int n_seqs) { return n_rows / kKvBlock + 2ll * n_seqs; }
-
 // What a wave knows of the first 64 sequences, a lane each: loaded together, so
 // that finding a row's or a slot's sequence costs one memory latency.
 struct KvLanes {
@@ -107,8 +101,70 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& v, const KvLanes& l, int s
   b = min(max(b, a), v.n_rows);
   return KvSeq{a, b - a, min(max(n, 0), v.max_pages * v.blocks * kKvBlock)};
 }
-__device__ __forceinline__ int kv_slot_key(const KvView& v, int i, int start) {
-  return min(max(start, 0), v.n_rows) / kKvBlock + 2 * i;
+// Sums over the lanes up to each one (DPP: within rows of 16, then rows).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int kv_dpp(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_sums(int x) {
+  x += kv_dpp<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
+  x += kv_dpp<0x112, 0xF>(x);
+  x += kv_dpp<0x114, 0xF>(x);
+  x += kv_dpp<0x118, 0xF>(x);
+  x += kv_dpp<0x142, 0xA>(x);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  x += kv_dpp<0x143, 0xC>(x);
+  return x;
+}
+
+// Slots: the blocks that a batch's rows touch, one after the other.  Up to 64
+// sequences are counted out exactly.  With more, sequence s has the slots from
+// row_start[s]/32 + 2 s on, at least as many as its m rows can touch ((m + 30)/32 + 1
+// rounded down), and the slots without a block do nothing.
+inline int64_t kv_slots(int n_rows, int n_seqs) {
+  if (n_seqs > 64) return n_rows / kKvBlock + 2ll * n_seqs;
+  const int64_t most = n_rows / kKvBlock + 2ll * n_seqs;
+  return most < n_rows ? most : n_rows;
+}
+struct KvBlock {
+  int s, block;  // sequence (-1: none) and block of it
+  bool first;    // its first slot
+  KvSeq q;
+};
+// empties: sequences whose rows all lie before position 0 have one slot too.
+__device__ __forceinline__ KvBlock kv_block_of(const KvView& v, const KvLanes& l, int slot,
+                                               bool empties = false) {
+  KvBlock k;
+  k.s = -1;
+  int local;
+  if (v.n_seqs <= 64) {
+    const int lane = (int)threadIdx.x & 63;
+    const int a = min(max(l.start, 0), v.n_rows), b = min(max(l.next, a), v.n_rows);
+    const int len = min(max(l.len, 0), v.max_pages * v.blocks * kKvBlock);
+    const int lo = max(len - (b - a), 0);
+    int n = b > a && len > lo ? (len - 1) / kKvBlock - lo / kKvBlock + 1 : 0;
+    if (empties && b > a && n == 0) n = 1;
+    if (lane >= v.n_seqs) n = 0;
+    const int end = wave_sums(n);
+    const uint64_t hit = __ballot(slot >= end - n && slot < end);
+    if (hit == 0) return k;
+    k.s = __ffsll((unsigned long long)hit) - 1;
+    local = slot - __builtin_amdgcn_readlane(end - n, k.s);
+    k.q = kv_seq(v, l, k.s);
+  } else {
+    auto key = [&](int i, int start) { return min(max(start, 0), v.n_rows) / kKvBlock + 2 * i; };
+    const int s = kv_find(v, l, [&](int i, int next) { return key(i + 1, next) <= slot; });
+    if (s >= v.n_seqs) return k;
+    k.q = kv_seq(v, l, s);
+    local = slot - key(s, k.q.row0);
+    const int lo = max(k.q.len - k.q.count, 0);
+    if (k.q.count == 0 || (lo / kKvBlock + local) * kKvBlock >= k.q.len) {
+      if (!empties || k.q.count == 0 || local) return k;
+    }
+    k.s = s;
+  }
+  k.first = local == 0;
+  k.block = max(k.q.len - k.q.count, 0) / kKvBlock + local;
+  return k;
 }
 
 }  // namespace plh

@@ -78,12 +78,13 @@ struct AppendArgs {
   int block_wgs;   // workgroups of the slots; those behind them rotate q rows
   int q_rows;      // rows of such a workgroup (1..kQRows)
   int rope;        // rotate
-  int k_vec, v_vec;  // float4 reads of k rows; of their partners by half a head too
-  int half_vec;
+  int k_vec;         // float4 reads of k rows
+  int tab_vec, half_vec;  // ... of the tables; of a k row's partners too
   RopeRows r;      // the tables, and q
 };
 
 constexpr int kQRows = 4;
+enum { PLAIN, LLAMA, QWEN };  // how a kernel rotates
 
 // x / s rounded to the nearest integer, ties to even, as the 64-bit quotient
 // rounds: x times the fp32 reciprocal is within 3e-5 of the quotient (|quotient|
@@ -110,66 +111,99 @@ __device__ __forceinline__ float wave_amax(float x) {
   return x;
 }
 
-// Eight elements of a row from d on, zeros from D on.
-__device__ __forceinline__ void load8(const float* row, int d, int D, int vec, float (&x)[8]) {
+// Loads stay where they are written: all of a row's before the first use (the
+// compiler otherwise puts each into a branch of its own, one latency after the
+// other).
+template <int N>
+__device__ __forceinline__ void here(float (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[n]));
+}
+
+// N elements of a row from d on, inside it (D elements) whatever d is.
+template <int N>
+__device__ __forceinline__ void load_n(const float* row, int d, int D, int vec, float (&x)[N]) {
   if (vec) {
-    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4 a = d < D ? *(const float4*)(row + d) : z;
-    const float4 b = d + 4 < D ? *(const float4*)(row + d + 4) : z;
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+#pragma unroll
+    for (int n = 0; n < N; n += 4) {
+      const float4 a = *(const float4*)(row + min(d + n, D - 4));
+      x[n] = a.x, x[n + 1] = a.y, x[n + 2] = a.z, x[n + 3] = a.w;
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = d + j < D ? row[d + j] : 0.0f;
+    for (int n = 0; n < N; ++n) x[n] = row[min(d + n, D - 1)];
   }
 }
 
-// Elements d..d+7 of a k row, rotated to position pos.
-__device__ __forceinline__ void load_k8(const AppendArgs& a, const float* row, int d, int pos,
-                                        float (&x)[8]) {
-  load8(row, d, a.v.D, a.k_vec, x);
-  if (!a.rope || d >= a.r.rot) return;
-  const int half = a.r.rot / 2;
-  const bool known = pos < a.r.n_pos;
-  const size_t tab = (size_t)(known ? pos : 0) * half;
-  const float nan = __builtin_nanf("");
-  if (!a.r.qwen) {
+// What turns a k row's elements 32 (c0 + t) + 8 g + j: the tables' entries and, in
+// half-split pairs, the elements' partners.
+template <int N, int MODE>
+struct Turn {
+  float y[N][8], c[N][8], s[N][8];
+  bool known;
+
+  __device__ __forceinline__ void load(const AppendArgs& a, const float* row, int c0, int g,
+                                       int pos) {
+    const int rot = a.r.rot, half = rot / 2;
+    known = pos < a.r.n_pos;
+    const int64_t tab = (int64_t)(known ? pos : 0) * half;
+    const float* cos_t = a.r.cos_t + tab;
+    const float* sin_t = a.r.sin_t + tab;
 #pragma unroll
-    for (int j = 0; j < 8; j += 2)
-      if (d + j < a.r.rot) {
-        const int i = (d + j) / 2;
-        rotate_pair(x[j], x[j + 1], known ? a.r.cos_t[tab + i] : nan,
-                    known ? a.r.sin_t[tab + i] : nan);
+    for (int t = 0; t < N; ++t) {
+      const int d = 32 * (c0 + t) + 8 * g;
+      if (MODE == LLAMA) {
+        float c4[4], s4[4];
+        load_n(cos_t, d / 2, half, a.tab_vec, c4);
+        load_n(sin_t, d / 2, half, a.tab_vec, s4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[t][j] = c4[j], s[t][j] = s4[j];
+      } else if (a.half_vec) {  // half is a multiple of 8: all eight on one side of it
+        const int e = min(d, rot - 8);
+        const bool lo = e < half;
+        load_n(row, lo ? e + half : e - half, a.v.D, 1, y[t]);
+        load_n(cos_t, lo ? e : e - half, half, 1, c[t]);
+        load_n(sin_t, lo ? e : e - half, half, 1, s[t]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int e = min(d + j, rot - 1), k = e < half ? e : e - half;
+          y[t][j] = row[e < half ? e + half : e - half];
+          c[t][j] = cos_t[k], s[t][j] = sin_t[k];
+        }
       }
-    return;
-  }
-  // the partner of element e lies half a rotated part away
-  float y[8], c[8], s[8];
-  if (a.half_vec) {  // half is a multiple of 8: all eight on one side of it
-    const bool lo = d < half;
-    const int i = lo ? d : d - half;
-    load8(row, lo ? d + half : d - half, a.v.D, 1, y);
-    load8(a.r.cos_t + tab, i, half, 1, c);
-    load8(a.r.sin_t + tab, i, half, 1, s);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int e = d + j, i = e < half ? e : e - half;
-      const bool in = e < a.r.rot;
-      y[j] = in ? row[e < half ? e + half : e - half] : 0.0f;
-      c[j] = in ? a.r.cos_t[tab + i] : 1.0f;
-      s[j] = in ? a.r.sin_t[tab + i] : 0.0f;
     }
   }
+
+  __device__ __forceinline__ void apply(const AppendArgs& a, int c0, int g, float (&x)[N][8]) {
+    const int rot = a.r.rot, half = rot / 2;
+    const float nan = __builtin_nanf("");
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = d + j;
-    if (e >= a.r.rot) continue;
-    float x0 = e < half ? x[j] : y[j], x1 = e < half ? y[j] : x[j];
-    rotate_pair(x0, x1, known ? c[j] : nan, known ? s[j] : nan);
-    x[j] = e < half ? x0 : x1;
+    for (int t = 0; t < N; ++t) {
+      const int d = 32 * (c0 + t) + 8 * g;
+      if (MODE == LLAMA) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x0 = x[t][2 * j], x1 = x[t][2 * j + 1];
+          rotate_pair(x0, x1, known ? c[t][j] : nan, known ? s[t][j] : nan);
+          const bool in = d + 2 * j < rot;
+          x[t][2 * j] = in ? x0 : x[t][2 * j], x[t][2 * j + 1] = in ? x1 : x[t][2 * j + 1];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          // (the pair's output that this element is: rotate_pair's bits, as products
+          // of two fp32 values are exact)
+          const int e = d + j;
+          const double sn = known ? (e < half ? -s[t][j] : s[t][j]) : nan;
+          const double cs = known ? c[t][j] : nan;
+          const float r = (float)__builtin_fma((double)x[t][j], cs, (double)y[t][j] * sn);
+          x[t][j] = e >= rot ? x[t][j] : r;
+        }
+      }
+    }
   }
-}
+};
 
 // A block's place and its new rows.
 struct Place {
@@ -195,6 +229,40 @@ struct Scale {
   __device__ __forceinline__ int code(float x) const { return zero ? 0 : quant(x, now, inv); }
 };
 
+// Sixteen values of a lane as codes.  x times the reciprocal plus 1.5 * 2^23 rounds
+// to the nearest integer, ties to even, and has it in its low byte; the
+// reciprocal's rounding moves a quotient below 128 by less than 1e-5, so only
+// where a wave has a value that near a tie (one wave in fifty) are all of them
+// taken from 64-bit quotients.
+__device__ __forceinline__ void codes16(const float (&x)[16], const Scale& s, uint32_t (&w)[4]) {
+  constexpr float kMagic = 12582912.0f;
+  float worst = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = x[4 * q + e], n = __builtin_fmaf(y, s.inv, kMagic);
+      worst = vmax(worst, __builtin_fabsf(__builtin_fmaf(y, s.inv, -(n - kMagic))));
+      t[e] = __float_as_uint(n);
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(t[3], t[2], 0x0C0C0400u);
+    w[q] = lo | hi << 16;
+  }
+  if (s.zero) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = 0;
+  } else if (__any(!(worst < 0.49998f))) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      w[q] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[q] |= (uint32_t)(s.code(x[4 * q + e]) & 0xFF) << (8 * e);
+    }
+  }
+}
+
 // Sixteen codes of a lane rounded again.
 __device__ __forceinline__ uint4 requant16(uint4 old, const Scale& s) {
   uint32_t w[4] = {old.x, old.y, old.z, old.w};
@@ -213,7 +281,7 @@ __device__ __forceinline__ uint4 requant16(uint4 old, const Scale& s) {
 // One new row in a block (a single token): two elements a lane at a time, the pairs
 // that rotate together, and single bytes stored.  The block's tiles are only
 // touched where its scale grows, or cleared where the row begins it.
-template <int DT>
+template <int DT, int MODE>
 __device__ __forceinline__ void append_row(const AppendArgs& a, const Place& p, uint4* tiles,
                                            float* scale, bool may_store) {
   constexpr int kPairs = (16 * DT + 63) / 64;  // of a lane
@@ -224,7 +292,7 @@ __device__ __forceinline__ void append_row(const AppendArgs& a, const Place& p, 
                              : a.k + (int64_t)(p.row0 + pos - p.start) * a.k_stride) +
                      p.head * D;
   const float was = older ? *scale : 0.0f;
-  const bool turn = !p.is_v && a.rope;
+  const bool turn = !p.is_v && MODE != PLAIN;
   const int rot = turn ? a.r.rot : 0, half = rot / 2;
   const bool known = pos < a.r.n_pos;
   const int64_t tab = (int64_t)(known ? pos : 0) * half;
@@ -235,8 +303,8 @@ __device__ __forceinline__ void append_row(const AppendArgs& a, const Place& p, 
   for (int n = 0; n < kPairs; ++n) {
     const int i = lane + 64 * n;
     const bool in = i < D / 2, rotates = i < half;
-    d[n][0] = rotates && a.r.qwen ? i : 2 * i;
-    d[n][1] = rotates && a.r.qwen ? i + half : 2 * i + 1;
+    d[n][0] = rotates && MODE == QWEN ? i : 2 * i;
+    d[n][1] = rotates && MODE == QWEN ? i + half : 2 * i + 1;
     x[n][0] = in ? row[d[n][0]] : 0.0f;
     x[n][1] = in ? row[d[n][1]] : 0.0f;
     if (rotates) {
@@ -281,99 +349,172 @@ __device__ __forceinline__ void append_row(const AppendArgs& a, const Place& p, 
   if (lane == 0) *scale = s.now;
 }
 
-// Several new rows: in registers in the order of the tiles (so each lane ends
-// with 16 adjacent bytes of every tile).  Blocks with older rows read their tiles
-// and put them back whole.
+// How the four waves of a workgroup share its jobs (a block of a kv head's k or v):
+// a wave a tile, two tiles of wide heads.
 template <int DT>
-__device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p, const int32_t* entry,
-                                            int b) {
+struct Share {
+  static constexpr int kWaves = DT < 4 ? (DT == 3 ? 4 : DT) : 4;  // of a job
+  static constexpr int kTiles = (DT + 3) / 4;                     // of a wave
+  static constexpr int kJobs = 4 / kWaves;                        // of a workgroup
+};
+
+// Several new rows: a wave's tiles of them in registers in the order of the codes (so
+// each lane ends with 16 adjacent bytes of every tile); the waves of a job
+// exchange their largest magnitudes.  Blocks with older rows read their tiles and
+// put them back whole.
+template <int DT, int MODE>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p, bool active,
+                                            const int32_t* entry, int b, float* red) {
+  constexpr int T = Share<DT>::kTiles;
   const KvView& v = a.v;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int c0 = wave % Share<DT>::kWaves * T;
   const bool older = p.lo > p.t0;
+  active = active && c0 < DT;
   const int page = *entry;
-  // x[c][8 h + j]: the element whose code is byte 8 h + j of this lane's sixteen
-  float x[DT][16];
-  if (!p.is_v) {
+  // The page's count, the scale and old tiles are asked for as soon as its number
+  // is there, while the rows are on their way.
+  const bool in_cache = page >= 0 && page < v.n_pages;
+  uint4 old[T];
+  float was = 0.0f;
+  int sharers = 0;
+  uint4* tiles = nullptr;
+  float* scale = nullptr;
+  auto ask = [&]() {
+    const int at = in_cache ? page : 0, unit = (p.head * v.blocks + b) * 2 + p.is_v;
+    tiles = (uint4*)(v.codes + at * v.page_codes + (int64_t)unit * DT * kKvTile);
+    scale = v.scales + at * v.page_scales + unit;
+    sharers = v.refs[at];
+#pragma unroll
+    for (int t = 0; t < T; ++t) old[t] = make_uint4(0u, 0u, 0u, 0u);
+    if (older && active) {
+      was = *scale;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        if (c0 + t < DT) old[t] = tiles[(c0 + t) * 64 + lane];
+    }
+  };
+  // x[t][8 h + j]: the element whose code is byte 8 h + j of this lane's sixteen of
+  // tile c0 + t (rows that are not new: a new one's, not used)
+  float x[T][16];
+  float amax = 0.0f;
+  if (!active) {
+  } else if (!p.is_v) {
+    float y[2][T][8];
+    const float* row[2];
+    int at[2];
+    Turn<T, MODE> turn[2];
+    const bool turns = MODE != PLAIN && 32 * c0 < a.r.rot;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int pos = p.t0 + 16 * h + i;
-      const bool fresh = pos >= p.lo && pos < p.len;
-      const float* row = a.k + (int64_t)(p.row0 + (fresh ? pos : p.lo) - p.start) * a.k_stride +
-                         p.head * v.D;
+      at[h] = min(max(pos, p.lo), p.len - 1);
+      row[h] = a.k + (int64_t)(p.row0 + at[h] - p.start) * a.k_stride + p.head * v.D;
 #pragma unroll
-      for (int c = 0; c < DT; ++c) {
-        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (fresh) load_k8(a, row, 32 * c + 8 * g, pos, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[c][8 * h + j] = y[j];
-      }
+      for (int t = 0; t < T; ++t) load_n(row[h], 32 * (c0 + t) + 8 * g, v.D, a.k_vec, y[h][t]);
     }
+    // (half-split pairs take three times the registers: one token at a time)
+    if (turns) turn[0].load(a, row[0], c0, g, at[0]);
+    if (turns && MODE == LLAMA) turn[1].load(a, row[1], c0, g, at[1]);
+    ask();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < T; ++t) here(y[h][t]);
+    if (turns) {
+      turn[0].apply(a, c0, g, y[0]);
+      if (MODE == QWEN) turn[1].load(a, row[1], c0, g, at[1]);
+      turn[1].apply(a, c0, g, y[1]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[t][8 * h + j] = y[h][t][j];
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int pos = p.t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-      const bool fresh = pos >= p.lo && pos < p.len;
-      const float* row = a.vv + (int64_t)(p.row0 + (fresh ? pos : p.lo) - p.start) * a.v_stride +
-                         p.head * v.D;
+      const int pos = min(max(p.t0 + 16 * (j >> 2) + 4 * g + (j & 3), p.lo), p.len - 1);
+      const float* row = a.vv + (int64_t)(p.row0 + pos - p.start) * a.v_stride + p.head * v.D;
 #pragma unroll
-      for (int c = 0; c < DT; ++c)
+      for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int d = 32 * c + 16 * h + i;
-          x[c][8 * h + j] = fresh && d < v.D ? row[d] : 0.0f;
+        for (int h = 0; h < 2; ++h)
+          x[t][8 * h + j] = row[min(32 * (c0 + t) + 16 * h + i, v.D - 1)];
+    }
+    ask();
+#pragma unroll
+    for (int t = 0; t < T; ++t) here(x[t]);
+  }
+  if (active) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int c = 32 * (c0 + t);
+      if (c + 32 > v.D) {  // elements behind D
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const int d = p.is_v ? c + 16 * (n >> 3) + i : c + 8 * g + (n & 7);
+          x[t][n] = d < v.D ? x[t][n] : 0.0f;
         }
+      }
+#pragma unroll
+      for (int n = 0; n < 16; ++n) amax = vmax(amax, __builtin_fabsf(x[t][n]));
     }
   }
-  if (page < 0 || page >= v.n_pages || v.refs[page] != 1) return;
-  const int unit = (p.head * v.blocks + b) * 2 + p.is_v;
-  uint4* tiles = (uint4*)(v.codes + page * v.page_codes + (int64_t)unit * DT * kKvTile);
-  float* scale = v.scales + page * v.page_scales + unit;
-  uint4 old[DT];
-  float was = 0.0f;
-  if (older) {
-    was = *scale;
+  amax = wave_amax(amax);
+  if (Share<DT>::kWaves > 1) {
+    if (lane == 0) red[wave] = amax;
+    __syncthreads();
+    const int w0 = wave / Share<DT>::kWaves * Share<DT>::kWaves;
 #pragma unroll
-    for (int c = 0; c < DT; ++c) old[c] = tiles[c * 64 + lane];
-  } else {
-#pragma unroll
-    for (int c = 0; c < DT; ++c) old[c] = make_uint4(0u, 0u, 0u, 0u);
+    for (int w = 0; w < Share<DT>::kWaves; ++w) amax = vmax(amax, red[w0 + w]);
   }
-  float amax = 0.0f;
+  if (!active || !in_cache || sharers != 1) return;
+  const Scale s(amax, was, older);
+  // which bytes are new rows': k's lane has tokens i and 16 + i, v's 4 g + (0..3) and
+  // 16 + those
+  uint32_t mask[2];
 #pragma unroll
-  for (int c = 0; c < DT; ++c)
+  for (int h = 0; h < 2; ++h) {
+    mask[h] = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) amax = vmax(amax, __builtin_fabsf(x[c][j]));
-  const Scale s(wave_amax(amax), was, older);
+    for (int e = 0; e < 4; ++e) {
+      const int u = p.t0 + 16 * h + (p.is_v ? 4 * g + e : i);
+      mask[h] |= u >= p.lo && u < p.len ? 0xFFu << (8 * e) : 0u;
+    }
+  }
 #pragma unroll
-  for (int c = 0; c < DT; ++c) {
-    const uint4 kept = s.grown ? requant16(old[c], s) : old[c];
-    uint32_t w[4] = {kept.x, kept.y, kept.z, kept.w};
+  for (int t = 0; t < T; ++t) {
+    if (c0 + t >= DT) continue;
+    const uint4 kept = s.grown ? requant16(old[t], s) : old[t];
+    const uint32_t k4[4] = {kept.x, kept.y, kept.z, kept.w};
+    uint32_t w[4];
+    codes16(x[t], s, w);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = 4 * q + e, h = n >> 3, j = n & 7;
-        const int t = p.is_v ? 16 * (j >> 2) + 4 * g + (j & 3) : 16 * h + i;
-        const bool fresh = p.t0 + t >= p.lo && p.t0 + t < p.len;
-        const uint32_t code = (uint32_t)(s.code(x[c][n]) & 0xFF) << (8 * e);
-        w[q] = fresh ? (w[q] & ~(0xFFu << (8 * e))) | code : w[q];
-      }
+      const uint32_t m = p.is_v ? mask[q & 1] : mask[q >> 1];
+      w[q] = (w[q] & m) | (k4[q] & ~m);
     }
-    tiles[c * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+    tiles[(c0 + t) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (lane == 0) *scale = s.now;
+  if (lane == 0 && c0 == 0) *scale = s.now;
 }
 
-// A wave per touched block, kv head and k or v (their rows' largest magnitude, the
-// scale, the codes), and behind them workgroups that rotate q rows.
+// The waves of a workgroup share a touched block's jobs (a kv head's k or v: its
+// rows' largest magnitude, the scale, the codes); workgroups behind the blocks'
+// rotate q rows.
 //
 // HBM bounds prompts (4 bytes read and 1 written an element); single tokens are
 // three memory latencies: row_start with len, the row with the page number, the
 // page's count and scale.
-template <int DT>
-__global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
+template <int DT, int MODE>
+__global__ __launch_bounds__(kKvThreads, DT > 4 ? 2 : MODE == QWEN ? 5 : 6) void
+kv8_append_kernel(AppendArgs a) {
+  __shared__ float red[4];
   const KvView& v = a.v;
-  if ((int)blockIdx.x >= a.block_wgs) {
+  if (MODE != PLAIN && (int)blockIdx.x >= a.block_wgs) {
     const int wg = (int)blockIdx.x - a.block_wgs;
     const int group = (int)fdiv((uint32_t)wg, a.r.fd_chunk);
     const int item = (wg - group * a.r.chunks) * kRopeThreads + (int)threadIdx.x;
@@ -383,7 +524,8 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
 #pragma unroll
     for (int n = 0; n < kQRows; ++n) {
       const int64_t row = (int64_t)group * a.q_rows + n;
-      if (n < a.q_rows && row < v.n_rows && item < a.r.per_row) it[n] = rope_load(a.r, row, item);
+      if (n < a.q_rows && row < v.n_rows && item < a.r.per_row) 
+        it[n] = rope_load<MODE == QWEN>(a.r, row, item);
     }
 #pragma unroll
     for (int n = 0; n < kQRows; ++n) {
@@ -393,36 +535,36 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(AppendArgs a) {
       if (s >= v.n_seqs || row < first) continue;
       const KvSeq q = kv_seq(v, lanes, s);
       const int pos = q.len - q.count + (int)row - q.row0;
-      if (pos >= 0 && item < a.r.per_row) rope_store(a.r, it[n], pos);
+      if (pos >= 0 && item < a.r.per_row) rope_store<MODE == QWEN>(a.r, it[n], pos);
     }
     return;
   }
+  // everything but the job is the same for the workgroup
   const int slot = (int)fdiv(blockIdx.x, a.fd_groups);
-  const int job = ((int)blockIdx.x - slot * a.groups) * 4 +
-                  __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int job = ((int)blockIdx.x - slot * a.groups) * Share<DT>::kJobs +
+                  wave / Share<DT>::kWaves;
   const KvLanes lanes = kv_lanes(v);
-  const int s =
-      kv_find(v, lanes, [&](int i, int next) { return kv_slot_key(v, i + 1, next) <= slot; });
-  if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
-  const KvSeq q = kv_seq(v, lanes, s);
+  const KvBlock k = kv_block_of(v, lanes, slot);
+  if (k.s < 0) return;
   Place p;
-  p.row0 = q.row0, p.len = q.len;
-  p.start = q.len - q.count;  // negative: rows before position 0 are dropped
+  p.row0 = k.q.row0, p.len = k.q.len;
+  p.start = k.q.len - k.q.count;  // negative: rows before position 0 are dropped
   p.lo = max(p.start, 0);
-  const int blk = p.lo / kKvBlock + slot - kv_slot_key(v, s, q.row0);
-  p.t0 = blk * kKvBlock;
-  if (q.count == 0 || p.t0 >= q.len) return;
-  p.head = job >> 1, p.is_v = job & 1;
-  const int e = (int)fdiv((uint32_t)blk, v.fd_blocks), b = blk - e * v.blocks;
-  const int32_t* entry = v.table + (size_t)s * v.max_pages + e;
+  p.t0 = k.block * kKvBlock;
+  const bool active = job < 2 * v.n_kv_heads;
+  p.head = active ? job >> 1 : 0, p.is_v = job & 1;
+  const int e = (int)fdiv((uint32_t)k.block, v.fd_blocks), b = k.block - e * v.blocks;
+  const int32_t* entry = v.table + (size_t)k.s * v.max_pages + e;
   if (min(p.len, p.t0 + kKvBlock) - max(p.lo, p.t0) > 1) {
-    append_rows<DT>(a, p, entry, b);
+    append_rows<DT, MODE>(a, p, active, entry, b, red);
     return;
   }
+  if (!active || wave % Share<DT>::kWaves) return;
   const int page = *entry;
   const bool ok = page >= 0 && page < v.n_pages;
   const int at = ok ? page : 0, unit = (p.head * v.blocks + b) * 2 + p.is_v;
-  append_row<DT>(a, p, (uint4*)(v.codes + at * v.page_codes + (int64_t)unit * DT * kKvTile),
+  append_row<DT, MODE>(a, p, (uint4*)(v.codes + at * v.page_codes + (int64_t)unit * DT * kKvTile),
                  v.scales + at * v.page_scales + unit, ok && v.refs[at] == 1);
 }
 
@@ -443,25 +585,21 @@ __global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
   const int job = ((int)blockIdx.x - slot * a.groups) * 4 +
                   __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const KvLanes lanes = kv_lanes(v);
-  const int s =
-      kv_find(v, lanes, [&](int i, int next) { return kv_slot_key(v, i + 1, next) <= slot; });
-  if (s >= v.n_seqs || job >= 2 * v.n_kv_heads) return;
-  const KvSeq q = kv_seq(v, lanes, s);
-  const int row0 = q.row0, count = q.count, len = q.len;
-  if (count == 0) return;
+  const KvBlock kb = kv_block_of(v, lanes, slot, true);
+  if (kb.s < 0 || job >= 2 * v.n_kv_heads) return;
+  const int row0 = kb.q.row0, count = kb.q.count, len = kb.q.len;
   const int start = len - count, lo = max(start, 0);
   const int head = job >> 1, is_v = job & 1;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
   float* dst = (is_v ? a.vv : a.k) + head * v.D;
   const int stride = is_v ? a.v_stride : a.k_stride;
-  const int local = slot - kv_slot_key(v, s, row0);
-  if (start < 0 && local == 0) {  // rows before position 0
+  if (start < 0 && kb.first) {  // rows before position 0
     for (int r = 0; r < min(-start, count); ++r)
       for (int d = lane; d < v.D; d += 64) dst[(int64_t)(row0 + r) * stride + d] = 0.0f;
   }
-  const int blk = lo / kKvBlock + local;
+  const int blk = kb.block;
   if (blk * kKvBlock >= len) return;
-  const int page = kv_page(v, s, blk), src = page < 0 ? 0 : page;
+  const int page = kv_page(v, kb.s, blk), src = page < 0 ? 0 : page;
   const int b = blk - (int)fdiv((uint32_t)blk, v.fd_blocks) * v.blocks;
   const int unit = (head * v.blocks + b) * 2 + is_v;
   const uint4* tiles = (const uint4*)(v.codes + src * v.page_codes + (int64_t)unit * DT * kKvTile);
@@ -527,7 +665,13 @@ bool quads(const void* p, int stride, int D) {
 
 template <int DT>
 void launch_append(const AppendArgs& a, unsigned wgs) {
-  hipLaunchKernelGGL(kv8_append_kernel<DT>, dim3(wgs), dim3(kKvThreads), 0, ctx().stream, a);
+  const dim3 grid(wgs), block(kKvThreads);
+  if (!a.rope)
+    hipLaunchKernelGGL((kv8_append_kernel<DT, PLAIN>), grid, block, 0, ctx().stream, a);
+  else if (a.r.qwen)
+    hipLaunchKernelGGL((kv8_append_kernel<DT, QWEN>), grid, block, 0, ctx().stream, a);
+  else
+    hipLaunchKernelGGL((kv8_append_kernel<DT, LLAMA>), grid, block, 0, ctx().stream, a);
 }
 template <int DT>
 void launch_fetch(const FetchArgs& a, unsigned wgs) {
@@ -592,7 +736,9 @@ int plh_kv8_append(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int lay
     return -1;
   }
   a.k = k, a.vv = v, a.k_stride = k_stride, a.v_stride = v_stride;
-  a.groups = (2 * H + 3) / 4;
+  // (as Share<tiles>::kJobs)
+  const int jobs = kv_tiles(D) == 1 ? 4 : kv_tiles(D) == 2 ? 2 : 1;
+  a.groups = (2 * H + jobs - 1) / jobs;
   a.fd_groups = make_fastdiv((uint32_t)a.groups);
   a.k_vec = quads(k, k_stride, D);
   a.rope = rope != nullptr;
@@ -600,8 +746,9 @@ int plh_kv8_append(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int lay
   if (rope) {
     a.r = rope_rows_args(rope, D, q, n_heads, q_stride, q_out, q_out_stride, nullptr, 0, 0,
                          nullptr, 0);
-    a.half_vec = a.k_vec && rope->rot_dim % 16 == 0 &&
-                 (((uintptr_t)rope->cos_tab | (uintptr_t)rope->sin_tab) & 15) == 0;
+    const bool tab16 = (((uintptr_t)rope->cos_tab | (uintptr_t)rope->sin_tab) & 15) == 0;
+    a.tab_vec = tab16 && rope->rot_dim % 8 == 0;
+    a.half_vec = tab16 && a.k_vec && rope->rot_dim % 16 == 0;
   }
   a.block_wgs = (int)(wgs < INT_MAX ? wgs : INT_MAX);
   // Prompts: several rows' loads in flight a workgroup; while there are few rows,

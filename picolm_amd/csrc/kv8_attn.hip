@@ -121,28 +121,14 @@ struct PlanLds {
   int found[6];
 };
 
-// Sums over the lanes up to each one (DPP: within rows of 16, then rows).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp(int x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ int wave_sums(int x) {
-  x += dpp<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8
-  x += dpp<0x112, 0xF>(x);
-  x += dpp<0x114, 0xF>(x);
-  x += dpp<0x118, 0xF>(x);
-  x += dpp<0x142, 0xA>(x);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
-  x += dpp<0x143, 0xC>(x);
-  return x;
-}
 __device__ __forceinline__ float wave_sums(float x) {
   auto f = [](int i) { return __uint_as_float((uint32_t)i); };
-  x += f(dpp<0x111, 0xF>((int)__float_as_uint(x)));
-  x += f(dpp<0x112, 0xF>((int)__float_as_uint(x)));
-  x += f(dpp<0x114, 0xF>((int)__float_as_uint(x)));
-  x += f(dpp<0x118, 0xF>((int)__float_as_uint(x)));
-  x += f(dpp<0x142, 0xA>((int)__float_as_uint(x)));
-  x += f(dpp<0x143, 0xC>((int)__float_as_uint(x)));
+  x += f(kv_dpp<0x111, 0xF>((int)__float_as_uint(x)));
+  x += f(kv_dpp<0x112, 0xF>((int)__float_as_uint(x)));
+  x += f(kv_dpp<0x114, 0xF>((int)__float_as_uint(x)));
+  x += f(kv_dpp<0x118, 0xF>((int)__float_as_uint(x)));
+  x += f(kv_dpp<0x142, 0xA>((int)__float_as_uint(x)));
+  x += f(kv_dpp<0x143, 0xC>((int)__float_as_uint(x)));
   return x;
 }
 

@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kSmallTable = 8 * kPlanThreads;  // entries
 
 struct PageArgs {
   int8_t* codes;
@@ -30,15 +31,16 @@ struct PageArgs {
   int32_t* dst;
   int32_t* spare;  // free page numbers; compact: where a page goes; fork: the parents' rows
   int chunks;      // of a copied page
+  FastDiv fd_page; // page_tokens
 };
 
-constexpr int kCopyChunk = 64 * 1024;  // bytes of codes a workgroup copies at a time
+constexpr int kCopyChunk = 16 * 1024;  // bytes of codes a workgroup copies at a time
 
 __device__ __forceinline__ int seq_len(const PageArgs& a, int s) {
   return min(max(a.len[s], 0), a.max_pages * a.page_tokens);
 }
 __device__ __forceinline__ int pages_of(const PageArgs& a, int n) {
-  return (n + a.page_tokens - 1) / a.page_tokens;
+  return (int)fdiv((uint32_t)(n + a.page_tokens - 1), a.fd_page);
 }
 __device__ __forceinline__ bool in_cache(const PageArgs& a, int page) {
   return page >= 0 && page < a.n_pages;
@@ -95,6 +97,28 @@ __global__ __launch_bounds__(kKvThreads) void kv8_fork_write_kernel(PageArgs a) 
   if (threadIdx.x == 0) a.len[s] = len;
 }
 
+// Both in one workgroup, for tables of few entries: one launch.
+__global__ __launch_bounds__(kPlanThreads) void kv8_fork_small_kernel(PageArgs a) {
+  const int entries = a.n_seqs * a.max_pages;
+  for (int i = (int)threadIdx.x; i < entries; i += kPlanThreads) {
+    const int s = i / a.max_pages, e = i - s * a.max_pages, parent = parent_of(a, s);
+    if (parent < 0) continue;
+    const int old = a.table[i], p = a.table[(size_t)parent * a.max_pages + e];
+    const int len = seq_len(a, parent), n = pages_of(a, len), had = pages_of(a, seq_len(a, s));
+    if (e < had && in_cache(a, old)) atomicSub(a.refs + old, 1);
+    if (e < n && in_cache(a, p)) atomicAdd(a.refs + p, 1);
+    a.spare[i] = e < n ? p : e < had ? -1 : old;
+    if (e == 0) a.spare[entries + s] = len;
+  }
+  __syncthreads();
+  for (int i = (int)threadIdx.x; i < entries; i += kPlanThreads) {
+    const int s = i / a.max_pages;
+    if (parent_of(a, s) < 0) continue;
+    a.table[i] = a.spare[i];
+    if (i == s * a.max_pages) a.len[s] = a.spare[entries + s];
+  }
+}
+
 // Sum of the earlier threads' x (of a workgroup of kPlanThreads) and of all.
 // part: kPlanWaves + 1 values of LDS, free again once every thread returned.
 __device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t* part, int64_t& total) {
@@ -118,75 +142,114 @@ __device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t* part, int64_t& 
   return before + sum - x;
 }
 
+constexpr int kListed = 4096;  // free pages kept in LDS; more go to the workspace
+
 // extend: a thread per sequence finds what it needs, all of them walk refs
 // for the free pages of the lowest numbers until there are enough, and if so
 // hand them out.  One workgroup: the walk is 16 KB a step and ends early; a
-// pool of 64 K pages with its free ones last takes 16 steps.
+// pool of 64 K pages with its free ones last takes 16 steps.  Few sequences on
+// few pages (a decode step) are four memory latencies and two barriers: wish,
+// len and the first 4096 counts together; last pages; their counts; stores.
 __global__ __launch_bounds__(kPlanThreads) void kv8_extend_kernel(PageArgs a) {
   __shared__ int32_t last[kKvMaxSeqs], at[kKvMaxSeqs], from[kKvMaxSeqs], to[kKvMaxSeqs];
-  __shared__ int64_t part[kPlanWaves];
+  __shared__ int32_t list[kListed];
+  __shared__ int32_t sum_lo[kPlanWaves], sum_hi[kPlanWaves], sum_copy[kPlanWaves],
+      sum_free[kPlanWaves];
   __shared__ int over;
   const int s = (int)threadIdx.x, lane = s & 63, wave = s >> 6;
   const bool mine = s < a.n_seqs;
+  if (s == 0) over = INT_MAX;
   const int add = mine ? max(a.wish[s], 0) : 0;
   const int len = mine ? seq_len(a, s) : 0;
-  const int have = pages_of(a, len);
+  int count4[4];  // counts of the step's pages 4 s .. 4 s + 3
+#pragma unroll
+  for (int k = 0; k < 4; ++k) count4[k] = 4 * s + k < a.n_pages ? a.refs[4 * s + k] : 1;
+  const int full = (int)fdiv((uint32_t)len, a.fd_page), in_last = len - full * a.page_tokens;
+  const int have = full + (in_last > 0);
   const int64_t want64 = ((int64_t)len + add + a.page_tokens - 1) / a.page_tokens;
-  const int32_t* row = a.table + (size_t)(mine ? s : 0) * a.max_pages;
   int tail = -1;
-  if (add > 0 && len % a.page_tokens) {
-    tail = row[len / a.page_tokens];
+  if (add > 0 && in_last) {
+    tail = a.table[(size_t)s * a.max_pages + full];
     if (!in_cache(a, tail)) tail = -1;
   }
+  const int sharers = tail >= 0 ? a.refs[tail] : 0;
   last[s] = tail;
-  if (s == 0) over = INT_MAX;
   __syncthreads();
-  if (want64 > a.max_pages && add > 0) atomicMin(&over, s);
+  if (add > 0 && want64 > a.max_pages) atomicMin(&over, s);
   // the earlier sharers of this last page leave it to the later ones
   int before = 0;
-  if (tail >= 0)
+  if (sharers > 1)
     for (int j = 0; j < s; ++j) before += last[j] == tail;
-  const int copies = tail >= 0 && a.refs[tail] - before > 1;
+  const int copies = sharers - before > 1;
   const int64_t count = (add > 0 ? want64 - have : 0) + copies;
-  int64_t total, n_copies;
-  const int64_t first = plan_scan(count, part, total);
-  const int64_t copy_at = plan_scan(copies, part, n_copies);
-  const int first_over = over;  // written before the scans' barriers
-  int64_t found = 0;
-  if (first_over == INT_MAX)
-    for (int base = 0; base < a.n_pages && found < total; base += 4 * kPlanThreads) {
+  // sums over the sequences in two halves of 16 and more bits (counts are below
+  // 2^26), and over the first step's free pages
+  int n_free = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) n_free += count4[k] == 0;
+  const int c_lo = (int)(count & 0xFFFF), c_hi = (int)(min(count, (int64_t)1 << 36) >> 16);
+  int lo = wave_sums(c_lo), hi = wave_sums(c_hi), cp = wave_sums(copies), fr = wave_sums(n_free);
+  if (lane == 63) sum_lo[wave] = lo, sum_hi[wave] = hi, sum_copy[wave] = cp, sum_free[wave] = fr;
+  __syncthreads();
+  int64_t total = 0, first = 0;
+  int n_copies = 0, copy_at = 0, rank = 0, found = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    const int64_t x = ((int64_t)sum_hi[w] << 16) + sum_lo[w];
+    first += w < wave ? x : 0, total += x;
+    copy_at += w < wave ? sum_copy[w] : 0, n_copies += sum_copy[w];
+    rank += w < wave ? sum_free[w] : 0, found += sum_free[w];
+  }
+  first += ((int64_t)(hi - c_hi) << 16) + (lo - c_lo);
+  copy_at += cp - copies, rank += fr - n_free;
+  const int first_over = over;
+  auto keep = [&](int p0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (count4[k] == 0) {
+        if (rank < total) (rank < kListed ? list : a.spare)[rank] = p0 + k;
+        ++rank;
+      }
+  };
+  if (first_over == INT_MAX) {
+    keep(4 * s);
+    for (int base = 4 * kPlanThreads; base < a.n_pages && found < total;
+         base += 4 * kPlanThreads) {
       const int p0 = base + 4 * s;
-      int free4[4], n = 0;
+      n_free = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        free4[k] = p0 + k < a.n_pages && a.refs[p0 + k] == 0;
-        n += free4[k];
+        count4[k] = p0 + k < a.n_pages ? a.refs[p0 + k] : 1;
+        n_free += count4[k] == 0;
       }
-      int64_t all;
-      int64_t rank = found + plan_scan(n, part, all);
+      fr = wave_sums(n_free);
+      __syncthreads();
+      if (lane == 63) sum_free[wave] = fr;
+      __syncthreads();
+      rank = found + fr - n_free;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (free4[k]) {
-          if (rank < total) a.spare[rank] = p0 + k;
-          ++rank;
-        }
-      found += all;
+      for (int w = 0; w < kPlanWaves; ++w) {
+        rank += w < wave ? sum_free[w] : 0;
+        found += sum_free[w];
+      }
+      keep(p0);
     }
+  }
   const bool ok = first_over == INT_MAX && found >= total;
   if (s == 0) {
     a.status[0] = first_over == INT_MAX && found < total
-                      ? (int)(total - found < INT_MAX ? total - found : INT_MAX)
+                      ? (int)min(total - found, (int64_t)INT_MAX)
                       : 0;
     a.status[1] = first_over == INT_MAX ? 0 : first_over + 1;
-    a.head[0] = ok ? (int)n_copies : 0;
+    a.head[0] = ok ? n_copies : 0;
   }
   if (!ok) return;  // the same for every thread
-  const int want = (int)want64;
-  at[s] = (int)(first + copies), from[s] = have, to[s] = add > 0 ? want : have;
-  __syncthreads();  // spare and the LDS are whole (this workgroup wrote them)
+  at[s] = (int)(first + copies), from[s] = have, to[s] = add > 0 ? (int)want64 : have;
+  __syncthreads();  // the lists are whole (this workgroup wrote them)
+  auto listed = [&](int64_t n) { return n < kListed ? list[n] : a.spare[n]; };
   if (copies) {
-    const int p = a.spare[first];
-    a.table[(size_t)s * a.max_pages + len / a.page_tokens] = p;
+    const int p = listed(first);
+    a.table[(size_t)s * a.max_pages + full] = p;
     a.refs[p] = 1;
     atomicSub(a.refs + tail, 1);
     a.src[copy_at] = tail, a.dst[copy_at] = p;
@@ -194,7 +257,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_extend_kernel(PageArgs a) {
   if (add > 0) a.len[s] = len + add;
   for (int q = wave; q < a.n_seqs; q += kPlanWaves)
     for (int e = from[q] + lane; e < to[q]; e += 64) {
-      const int p = a.spare[at[q] + e - from[q]];
+      const int p = listed(at[q] + (int64_t)(e - from[q]));
       a.table[(size_t)q * a.max_pages + e] = p;
       a.refs[p] = 1;
     }
@@ -260,13 +323,13 @@ __global__ __launch_bounds__(kKvThreads) void kv8_copy_kernel(PageArgs a, int re
     uint4* y = (uint4*)(a.codes + to * a.page_codes);
     const int end = min((chunk + 1) * (kCopyChunk / 16), (int)(a.page_codes / 16));
     int i = chunk * (kCopyChunk / 16) + (int)threadIdx.x;
-    // eight loads in flight a thread
-    for (; i + 7 * kKvThreads < end; i += 8 * kKvThreads) {
-      uint4 r[8];
+    // four loads in flight a thread
+    for (; i + 3 * kKvThreads < end; i += 4 * kKvThreads) {
+      uint4 r[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] = x[i + k * kKvThreads];
+      for (int k = 0; k < 4; ++k) r[k] = x[i + k * kKvThreads];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y[i + k * kKvThreads] = r[k];
+      for (int k = 0; k < 4; ++k) y[i + k * kKvThreads] = r[k];
     }
     for (; i < end; i += kKvThreads) y[i] = x[i];
     if (chunk == 0) {
@@ -300,6 +363,7 @@ int page_args(const plh_kv8_cache* c, const plh_kv8_seqs* s, const int32_t* wish
   a.codes = c->codes, a.scales = c->scales;
   a.page_codes = (int64_t)(plh_kv8_code_bytes(c) / (size_t)c->n_pages);
   a.page_scales = (int64_t)(plh_kv8_scale_bytes(c) / (size_t)c->n_pages / sizeof(float));
+  a.fd_page = make_fastdiv((uint32_t)c->page_tokens);
   a.page_tokens = c->page_tokens, a.n_pages = c->n_pages;
   a.n_seqs = s->n_seqs, a.max_pages = s->max_pages;
   a.table = s->table, a.len = s->len, a.refs = s->refs;
@@ -313,8 +377,8 @@ int page_args(const plh_kv8_cache* c, const plh_kv8_seqs* s, const int32_t* wish
 }
 
 int launch_copies(const PageArgs& a, int64_t most, int remap) {
-  // enough workgroups for every CU to have four, or one an item
-  const int64_t items = most * a.chunks, full = 4ll * ctx().num_cus;
+  // enough workgroups for every CU to have eight, or one an item
+  const int64_t items = most * a.chunks, full = 8ll * ctx().num_cus;
   hipLaunchKernelGGL(kv8_copy_kernel, dim3((unsigned)(items < full ? items : full)),
                      dim3(kKvThreads), 0, ctx().stream, a, remap);
   return check_hip(hipGetLastError(), "kv8_copy_kernel");
@@ -341,6 +405,10 @@ int plh_kv8_fork(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, const int
                                  (size_t)(seqs->max_pages > 0 ? seqs->max_pages + 1ll : 0)
                            : 0;
   if (page_args(cache, seqs, parent, nullptr, true, false, 0, rows, "plh_kv8_fork", a)) return -1;
+  if ((int64_t)a.n_seqs * a.max_pages <= kSmallTable) {
+    hipLaunchKernelGGL(kv8_fork_small_kernel, dim3(1), dim3(kPlanThreads), 0, ctx().stream, a);
+    return check_hip(hipGetLastError(), "kv8_fork_small_kernel");
+  }
   hipLaunchKernelGGL(kv8_fork_count_kernel, dim3((unsigned)a.n_seqs), dim3(kKvThreads), 0,
                      ctx().stream, a);
   hipLaunchKernelGGL(kv8_fork_write_kernel, dim3((unsigned)a.n_seqs), dim3(kKvThreads), 0,

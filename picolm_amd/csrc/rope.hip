@@ -48,6 +48,7 @@ RopeRows rope_rows_args(const plh_rope* r, int head_dim, const float* q, int n_h
   a.per_head = a.pairs + (head_dim - a.rot) / v;
   a.per_row = (n_heads + n_kv_heads) * a.per_head;
   a.chunks = (a.per_row + kRopeThreads - 1) / kRopeThreads;
+  if (a.chunks < 1) a.chunks = 1;  // no heads: nothing is launched for them
   a.fd_head = make_fastdiv((uint32_t)a.per_head);
   a.fd_chunk = make_fastdiv((uint32_t)a.chunks);
   return a;
@@ -123,12 +124,13 @@ __global__ __launch_bounds__(256) void rope_tables_kernel(TableArgs a) {
 
 // A thread per item; the row's position arrives while its elements do.  HBM
 // bounds it: every element is read and written once.
+template <bool QWEN>
 __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeRows a, const int32_t* pos) {
   const int row = (int)fdiv(blockIdx.x, a.fd_chunk);
   const int item = ((int)blockIdx.x - row * a.chunks) * kRopeThreads + (int)threadIdx.x;
   if (item >= a.per_row) return;
   const int p = pos[row];
-  rope_store(a, rope_load(a, row, item), p);
+  rope_store<QWEN>(a, rope_load<QWEN>(a, row, item), p);
 }
 
 }  // namespace
@@ -257,8 +259,11 @@ int plh_rope_rows(const plh_rope* rope, int n_rows, const int32_t* pos, int head
   }
   if (rope_ready("plh_rope_rows")) return -1;
   if (!any) return 0;
-  hipLaunchKernelGGL(rope_rows_kernel, dim3((unsigned)n_rows * (unsigned)a.chunks),
-                     dim3(kRopeThreads), 0, ctx().stream, a, pos);
+  const dim3 grid((unsigned)n_rows * (unsigned)a.chunks), block(kRopeThreads);
+  if (a.qwen)
+    hipLaunchKernelGGL(rope_rows_kernel<true>, grid, block, 0, ctx().stream, a, pos);
+  else
+    hipLaunchKernelGGL(rope_rows_kernel<false>, grid, block, 0, ctx().stream, a, pos);
   return check_hip(hipGetLastError(), "rope_rows_kernel");
 }
 

@@ -47,6 +47,7 @@ struct RopeItem {
   int i;       // number in its head
   float4 x0, x1;
 };
+template <bool QWEN>
 __device__ __forceinline__ RopeItem rope_load(const RopeRows& a, int64_t row, int item) {
   RopeItem it;
   int head = (int)fdiv((uint32_t)item, a.fd_head);
@@ -65,15 +66,16 @@ __device__ __forceinline__ RopeItem rope_load(const RopeRows& a, int64_t row, in
     else
       it.x0.x = x[d];
   } else if (!a.vec) {
-    it.x0.x = x[a.qwen ? i : 2 * i];
-    it.x1.x = x[a.qwen ? i + a.rot / 2 : 2 * i + 1];
-  } else if (a.qwen) {
+    it.x0.x = x[QWEN ? i : 2 * i];
+    it.x1.x = x[QWEN ? i + a.rot / 2 : 2 * i + 1];
+  } else if (QWEN) {
     it.x0 = *(const float4*)(x + 4 * i), it.x1 = *(const float4*)(x + 4 * i + a.rot / 2);
   } else {
     it.x0 = *(const float4*)(x + 4 * i);
   }
   return it;
 }
+template <bool QWEN>
 __device__ __forceinline__ void rope_store(const RopeRows& a, RopeItem it, int pos) {
   const int i = it.i;
   float* y = it.y;
@@ -88,9 +90,9 @@ __device__ __forceinline__ void rope_store(const RopeRows& a, RopeItem it, int p
       y[d] = it.x0.x;
   } else if (!a.vec) {
     rotate_pair(it.x0.x, it.x1.x, known ? a.cos_t[tab + i] : nan, known ? a.sin_t[tab + i] : nan);
-    y[a.qwen ? i : 2 * i] = it.x0.x;
-    y[a.qwen ? i + a.rot / 2 : 2 * i + 1] = it.x1.x;
-  } else if (a.qwen) {
+    y[QWEN ? i : 2 * i] = it.x0.x;
+    y[QWEN ? i + a.rot / 2 : 2 * i + 1] = it.x1.x;
+  } else if (QWEN) {
     float4 c = *(const float4*)(a.cos_t + tab + 4 * i), s = *(const float4*)(a.sin_t + tab + 4 * i);
     if (!known) c = s = make_float4(nan, nan, nan, nan);
     rotate_pair(it.x0.x, it.x1.x, c.x, s.x);

@@ -426,6 +426,8 @@ def test_append_rotates(gpu, case, misaligned):
     q_out = run_append(P, dev, 0, rows, k, v, rope=rope, q=q, k_extra=pad, k_off=pad)
     dev.same_contents(case)
     assert np.array_equal(q_out, turned[1])
+    run_append(P, dev, 0, rows, k, v, rope=rope)  # k alone: the same again
+    dev.same_contents(case)
     dev.free()
 
 

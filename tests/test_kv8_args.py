@@ -245,6 +245,8 @@ def test_not_initialised():
         pytest.skip("a device is visible")
     refused(attn(), "not initialised")
     refused(append(), "not initialised")
+    refused(append(rope=tables()), "not initialised")  # no q rows to rotate
+    refused(append(n_rows=0, k=None, v=None), "not initialised")
     refused(rows(), "not initialised")
     refused(P.lib.plh_rope_tables(C.byref(spec().desc), 0, 4, FAKE, FAKE), "not initialised")
     refused(P.lib.plh_kv8_extend(C.byref(cache()), C.byref(seqs()), FAKE, FAKE), "not initialised")
