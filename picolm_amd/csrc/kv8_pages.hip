@@ -34,7 +34,14 @@ struct PageArgs {
   FastDiv fd_page; // page_tokens
 };
 
-constexpr int kCopyChunk = 16 * 1024;  // bytes of codes a workgroup copies at a time
+// A workgroup copies kCopyChunk bytes of codes at a time, kCopyLoads loads in
+// flight a thread.  Its stores pass L2 by: 16 copied pages of 704 KB take 12.5
+// us with their plan (13.4 through L2), 231 MB of moves 51 us (56; 4.5 TB/s,
+// what a large copy reaches).  One load a thread measures the same, eight 2%
+// more.
+constexpr int kCopyLoads = 4;
+constexpr int kCopyChunk = kCopyLoads * 16 * kKvThreads;
+typedef uint32_t Vec16 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ int seq_len(const PageArgs& a, int s) {
   return min(max(a.len[s], 0), a.max_pages * a.page_tokens);
@@ -315,28 +322,29 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_compact_kernel(PageArgs a) {
 // compact also follows the moves in the table.
 __global__ __launch_bounds__(kKvThreads) void kv8_copy_kernel(PageArgs a, int remap) {
   const int n = a.head[0];
-  const int64_t items = (int64_t)n * a.chunks;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int c = (int)(item / a.chunks), chunk = (int)(item - (int64_t)c * a.chunks);
+  // (page, chunk) advance by the grid's quotient and remainder
+  const int step_c = (int)gridDim.x / a.chunks, step_k = (int)gridDim.x - step_c * a.chunks;
+  int c = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - c * a.chunks;
+  while (c < n) {
     const int64_t from = a.src[c], to = a.dst[c];
-    const uint4* x = (const uint4*)(a.codes + from * a.page_codes);
-    uint4* y = (uint4*)(a.codes + to * a.page_codes);
-    const int end = min((chunk + 1) * (kCopyChunk / 16), (int)(a.page_codes / 16));
-    int i = chunk * (kCopyChunk / 16) + (int)threadIdx.x;
-    // four loads in flight a thread
-    for (; i + 3 * kKvThreads < end; i += 4 * kKvThreads) {
-      uint4 r[4];
+    const uint32_t at = (uint32_t)chunk * kCopyChunk + threadIdx.x * 16, end = (uint32_t)a.page_codes;
+    const int8_t* x = a.codes + from * a.page_codes + at;
+    int8_t* y = a.codes + to * a.page_codes + at;
+    Vec16 r[kCopyLoads];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r[k] = x[i + k * kKvThreads];
+    for (int k = 0; k < kCopyLoads; ++k)
+      if (at + k * 16 * kKvThreads < end) r[k] = *(const Vec16*)(x + k * 16 * kKvThreads);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[i + k * kKvThreads] = r[k];
-    }
-    for (; i < end; i += kKvThreads) y[i] = x[i];
+    for (int k = 0; k < kCopyLoads; ++k)
+      if (at + k * 16 * kKvThreads < end)
+        __builtin_nontemporal_store(r[k], (Vec16*)(y + k * 16 * kKvThreads));
     if (chunk == 0) {
       const float* sx = a.scales + from * a.page_scales;
       float* sy = a.scales + to * a.page_scales;
       for (int k = threadIdx.x; k < a.page_scales; k += kKvThreads) sy[k] = sx[k];
     }
+    c += step_c, chunk += step_k;
+    if (chunk >= a.chunks) chunk -= a.chunks, ++c;
   }
   if (!remap || n == 0) return;
   const int live = a.head[1];
