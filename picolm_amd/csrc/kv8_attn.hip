@@ -46,8 +46,8 @@ constexpr float kPlainMax = 65536.0f;  // log2 units: larger running maxima take
 // Weights (up to 2^8) times a v scale in units of 2^dO: exponents that leave both
 // fp16 parts their bits.
 constexpr int kUnitLo = -4, kUnitHi = 3;
-constexpr int kMinChunkShare = 32;    // blocks: a chunk's partials cost some ten blocks' time
-constexpr int kMinChunk = 16;         // blocks
+constexpr int kMinChunk = 16;      // blocks (a SHARE unit: for each of a wave's tiles, as its
+                                   // partial results grow with them)
 constexpr int kMaxTarget = 2048;   // most chunks asked for of the units that are cut
 
 // Arrival counters of cut units, zero between launches.
@@ -179,8 +179,9 @@ __device__ __forceinline__ int quota_of(const AttnArgs& a, float work) {
   return (int)fminf(q, 1e9f);
 }
 // Chunks of a sequence's units: a quota of work each, at least kMinChunk blocks.
+template <int CT>
 __device__ __forceinline__ int chunks_of(int len, int form, int quota) {
-  const int c = form == SHARE ? max(kMinChunkShare, quota / 4) : max(kMinChunk, quota);
+  const int c = form == SHARE ? max(kMinChunk * CT, quota / 4) : max(kMinChunk, quota);
   const int n = blocks_of(len);
   return c >= n ? 1 : (int)(((uint32_t)n + (uint32_t)c - 1) / (uint32_t)c);
 }
@@ -213,7 +214,7 @@ __device__ __forceinline__ Unit find_unit(const AttnArgs& a, int wg, PlanLds& ld
     const int64_t cols = (int64_t)u.rows * a.G;
     u.form = form_of<MIXED>(cols);
     const int uc = unit_cols<CT>(u.form), units = (int)((cols + uc - 1) / uc);
-    u.chunks = uniform(chunks_of(u.len, u.form, quota_of(a, work_of(units, u.len, u.form))));
+    u.chunks = uniform(chunks_of<CT>(u.len, u.form, quota_of(a, work_of(units, u.len, u.form))));
     if (wg >= (int64_t)units * u.chunks * v.n_kv_heads) return u;
     u.s = 0;
     place_unit<CT>(a, u, wg, 0);
@@ -232,7 +233,7 @@ __device__ __forceinline__ Unit find_unit(const AttnArgs& a, int wg, PlanLds& ld
     const float work = wave_sums(work_of(units, len, form));
     const int quota = quota_of(a, __uint_as_float((uint32_t)__builtin_amdgcn_readlane(
                                       (int)__float_as_uint(work), 63)));
-    const int n_chunks = chunks_of(len, form, quota);
+    const int n_chunks = chunks_of<CT>(len, form, quota);
     // (more than the grid: as good as one more, and 64 of them no overflow)
     const int64_t all = (int64_t)units * n_chunks * v.n_kv_heads;
     const int n_wgs = all > kMaxWorkgroups ? kMaxWorkgroups + 1 : (int)all;
@@ -281,7 +282,7 @@ __device__ __forceinline__ Unit find_unit(const AttnArgs& a, int wg, PlanLds& ld
   int n_wgs[4], n_chunks[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    n_chunks[k] = chunks_of(len[k], form[k], quota);
+    n_chunks[k] = chunks_of<CT>(len[k], form[k], quota);
     n_wgs[k] = units[k] * n_chunks[k] * v.n_kv_heads;
     wgs += n_wgs[k];
     cut += n_chunks[k] > 1 ? n_wgs[k] : 0;
@@ -955,15 +956,15 @@ __device__ __forceinline__ void attend_share(const AttnArgs& a, const Unit& u, h
   if (u.chunks > 1) res.join(merge, s_last);
 }
 
-// Waves a SIMD holds: what the registers of a column tile allow without spills.
-constexpr int waves_per_simd(int DT, bool mixed) {
-  return !mixed ? (DT <= 2 ? 4 : DT <= 3 ? 3 : DT <= 5 ? 2 : 1) : DT <= 2 ? 3 : DT <= 4 ? 2 : 1;
+// Waves a SIMD holds: what the registers of a wave's column tiles allow without
+// spills (tiles 0: single tokens only).
+constexpr int waves_per_simd(int DT, int tiles) {
+  return tiles == 2 ? (DT <= 2 ? 3 : DT <= 4 ? 2 : 1) : DT <= 2 ? 4 : DT <= 3 ? 3 : DT <= 5 ? 2 : 1;
 }
-constexpr int kShareTiles = 2;  // column tiles of a wave that shares its keys
 
 // Launches of sequences of up to 16 columns only, and any others.
 template <int DT>
-__global__ __launch_bounds__(kKvThreads, waves_per_simd(DT, false))
+__global__ __launch_bounds__(kKvThreads, waves_per_simd(DT, 0))
 void kv8_attn_tokens_kernel(AttnArgs a) {
   constexpr int kMerge = 2 * 16 * Sizes<DT>::kMergeRow, kJoin = 6 * kKvThreads;
   __shared__ PlanLds plan;
@@ -972,28 +973,30 @@ void kv8_attn_tokens_kernel(AttnArgs a) {
   const Unit u = find_unit<1, false>(a, (int)blockIdx.x, plan);
   if (u.s >= 0) attend_split<DT>(a, u, merge, s_last);
 }
-template <int DT>
-__global__ __launch_bounds__(kKvThreads, waves_per_simd(DT, true))
+template <int DT, int CT>
+__global__ __launch_bounds__(kKvThreads, waves_per_simd(DT, CT))
 void kv8_attn_mixed_kernel(AttnArgs a) {
   constexpr int kMerge = 2 * 16 * Sizes<DT>::kMergeRow, kJoin = 6 * kKvThreads;
   constexpr int kTiles = 2 * 2 * DT * 2 * 64 * 4;  // floats of the two buffers
   __shared__ PlanLds plan;
   __shared__ __align__(16) float lds[kTiles + kJoin > kMerge ? kTiles + kJoin : kMerge];
   __shared__ int s_last;
-  const Unit u = find_unit<kShareTiles, true>(a, (int)blockIdx.x, plan);
+  const Unit u = find_unit<CT, true>(a, (int)blockIdx.x, plan);
   if (u.s < 0) return;
   if (u.form == SPLIT)
     attend_split<DT>(a, u, lds, s_last);
   else
-    attend_share<DT, kShareTiles>(a, u, (half8_t*)lds, lds + kTiles, s_last);
+    attend_share<DT, CT>(a, u, (half8_t*)lds, lds + kTiles, s_last);
 }
 
+// tiles: 0 for the tokens kernel, else column tiles of a wave that shares its keys
 template <int DT>
-int launch_attn(AttnArgs& a, int n_heads, bool tokens) {
+int launch_attn(AttnArgs& a, int n_heads, int tiles) {
   const KvView& v = a.v;
-  const int cus = ctx().num_cus;
-  const int uc = tokens ? 16 : 64 * kShareTiles;
-  a.target = min(tokens ? 4 * cus : 3 * cus, kMaxTarget);
+  const int uc = tiles ? 64 * tiles : 16;
+  // As many chunks as run at once; twice as many of the larger units, which then end
+  // more evenly.
+  a.target = min((tiles == 2 ? 2 : 1) * waves_per_simd(DT, tiles) * ctx().num_cus, kMaxTarget);
   a.per_target = nextafterf(1.0f / (float)a.target, 1.0f);
   a.part_cols = uc;
   if (ensure_workspace((size_t)4 * a.target * uc * Sizes<DT>::kRow * sizeof(float))) return -1;
@@ -1010,10 +1013,12 @@ int launch_attn(AttnArgs& a, int n_heads, bool tokens) {
     return -1;
   }
   const dim3 grid((unsigned)wgs), block(kKvThreads);
-  if (tokens)
+  if (tiles == 0)
     hipLaunchKernelGGL(kv8_attn_tokens_kernel<DT>, grid, block, 0, ctx().stream, a);
+  else if (tiles == 1)
+    hipLaunchKernelGGL((kv8_attn_mixed_kernel<DT, 1>), grid, block, 0, ctx().stream, a);
   else
-    hipLaunchKernelGGL(kv8_attn_mixed_kernel<DT>, grid, block, 0, ctx().stream, a);
+    hipLaunchKernelGGL((kv8_attn_mixed_kernel<DT, 2>), grid, block, 0, ctx().stream, a);
   return check_hip(hipGetLastError(), "kv8_attn_kernel");
 }
 
@@ -1052,16 +1057,22 @@ extern "C" int plh_kv8_attn(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs
   a.out_vec = (((uintptr_t)out | (uintptr_t)out_stride * 4 | (uintptr_t)D * 4) & 15) == 0;
   a.fd_g = make_fastdiv((uint32_t)a.G);
   a.fd_kvh = make_fastdiv((uint32_t)cache->n_kv_heads);
-  // Short sequences (on average) in a launch of their own registers.
-  const bool tokens = (int64_t)n_rows * a.G <= 16ll * min(n_rows, seqs->n_seqs);
+  // Short sequences (on average) in a launch of their own registers.  Others' waves
+  // take two tiles of columns, so that keys are read from LDS half as often, where
+  // that leaves two units and more for every CU.
+  const int64_t seqs_rows = min(n_rows, seqs->n_seqs);
+  const bool tokens = (int64_t)n_rows * a.G <= 16 * seqs_rows;
+  const bool few = (int64_t)n_rows * n_heads / 128 + seqs_rows * cache->n_kv_heads <
+                   2ll * ctx().num_cus;
+  const int tiles = tokens ? 0 : few ? 1 : 2;
   switch (kv_tiles(D)) {
-    case 1: return launch_attn<1>(a, n_heads, tokens);
-    case 2: return launch_attn<2>(a, n_heads, tokens);
-    case 3: return launch_attn<3>(a, n_heads, tokens);
-    case 4: return launch_attn<4>(a, n_heads, tokens);
-    case 5: return launch_attn<5>(a, n_heads, tokens);
-    case 6: return launch_attn<6>(a, n_heads, tokens);
-    case 7: return launch_attn<7>(a, n_heads, tokens);
-    default: return launch_attn<8>(a, n_heads, tokens);
+    case 1: return launch_attn<1>(a, n_heads, tiles);
+    case 2: return launch_attn<2>(a, n_heads, tiles);
+    case 3: return launch_attn<3>(a, n_heads, tiles);
+    case 4: return launch_attn<4>(a, n_heads, tiles);
+    case 5: return launch_attn<5>(a, n_heads, tiles);
+    case 6: return launch_attn<6>(a, n_heads, tiles);
+    case 7: return launch_attn<7>(a, n_heads, tiles);
+    default: return launch_attn<8>(a, n_heads, tiles);
   }
 }
