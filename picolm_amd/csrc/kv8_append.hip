@@ -571,13 +571,30 @@ kv8_append_kernel(AppendArgs a) {
 struct FetchArgs {
   KvView v;
   float *k, *vv;
-  int k_stride, v_stride, k_vec;
+  int k_stride, v_stride, k_vec, v_vec;
   int groups;
   FastDiv fd_groups;
 };
 
-// A wave per block, kv head and k or v, as the append: 16 adjacent codes a lane
-// and tile.  HBM (the 4-byte values written) bounds it.
+__device__ __forceinline__ float code_of(uint32_t w, int byte) {
+  return (float)(int)(int8_t)(w >> (8 * byte));
+}
+// four elements of a row from d on, inside it
+__device__ __forceinline__ void store_four(float* row, int d, int D, int vec, float4 y) {
+  if (vec) {
+    if (d < D) *(float4*)(row + d) = y;
+  } else {
+    if (d < D) row[d] = y.x;
+    if (d + 1 < D) row[d + 1] = y.y;
+    if (d + 2 < D) row[d + 2] = y.z;
+    if (d + 3 < D) row[d + 3] = y.w;
+  }
+}
+
+// A wave per block, kv head, k or v and tile.  Of k a lane takes 16 adjacent bytes,
+// eight elements of two tokens; of v four words, four elements of four tokens: rows
+// are written 128 bytes at a time.  HBM (the 4-byte values written) bounds it, or for
+// few rows the latencies of lengths, page, codes and stores.
 template <int DT>
 __global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
   const KvView& v = a.v;
@@ -586,63 +603,58 @@ __global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
                   __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const KvLanes lanes = kv_lanes(v);
   const KvBlock kb = kv_block_of(v, lanes, slot, true);
-  if (kb.s < 0 || job >= 2 * v.n_kv_heads) return;
+  const int part = job / DT, c = job - part * DT;
+  if (kb.s < 0 || part >= 2 * v.n_kv_heads) return;
   const int row0 = kb.q.row0, count = kb.q.count, len = kb.q.len;
   const int start = len - count, lo = max(start, 0);
-  const int head = job >> 1, is_v = job & 1;
-  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-  float* dst = (is_v ? a.vv : a.k) + head * v.D;
-  const int stride = is_v ? a.v_stride : a.k_stride;
-  if (start < 0 && kb.first) {  // rows before position 0
+  const int head = part >> 1, is_v = part & 1;
+  const int lane = threadIdx.x & 63, D = v.D;
+  float* dst = (is_v ? a.vv : a.k) + head * D;
+  const int stride = is_v ? a.v_stride : a.k_stride, vec = is_v ? a.v_vec : a.k_vec;
+  if (start < 0 && kb.first && c == 0) {  // rows before position 0
     for (int r = 0; r < min(-start, count); ++r)
-      for (int d = lane; d < v.D; d += 64) dst[(int64_t)(row0 + r) * stride + d] = 0.0f;
+      for (int d = lane; d < D; d += 64) dst[(int64_t)(row0 + r) * stride + d] = 0.0f;
   }
   const int blk = kb.block;
   if (blk * kKvBlock >= len) return;
   const int page = kv_page(v, kb.s, blk), src = page < 0 ? 0 : page;
   const int b = blk - (int)fdiv((uint32_t)blk, v.fd_blocks) * v.blocks;
   const int unit = (head * v.blocks + b) * 2 + is_v;
-  const uint4* tiles = (const uint4*)(v.codes + src * v.page_codes + (int64_t)unit * DT * kKvTile);
-  const float scale = page < 0 ? __builtin_nanf("") : v.scales[src * v.page_scales + unit];
+  const int8_t* tile = v.codes + src * v.page_codes + ((int64_t)unit * DT + c) * kKvTile;
+  const float* sc = v.scales + src * v.page_scales + unit;
   const int t0 = blk * kKvBlock;
-  uint4 tile[DT];
+  auto row = [&](int t) { return dst + (int64_t)(row0 + t - start) * stride; };
+  if (!is_v) {
+    const int g = lane >> 4, i = lane & 15, d = 32 * c + 8 * g;
+    const uint4 w = ((const uint4*)tile)[lane];
+    const float s = page < 0 ? __builtin_nanf("") : *sc;
 #pragma unroll
-  for (int c = 0; c < DT; ++c) tile[c] = tiles[c * 64 + lane];
-#pragma unroll
-  for (int c = 0; c < DT; ++c) {
-    const uint32_t w[4] = {tile[c].x, tile[c].y, tile[c].z, tile[c].w};
-    float y[16];
-#pragma unroll
-    for (int n = 0; n < 16; ++n) y[n] = (float)(int)(int8_t)(w[n >> 2] >> (8 * (n & 3))) * scale;
-    if (!is_v) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int pos = t0 + 16 * h + i, d = 32 * c + 8 * g;
-        if (pos < lo || pos >= len) continue;
-        float* row = dst + (int64_t)(row0 + pos - start) * stride;
-        if (a.k_vec) {
-          if (d < v.D)
-            *(float4*)(row + d) = make_float4(y[8 * h], y[8 * h + 1], y[8 * h + 2], y[8 * h + 3]);
-          if (d + 4 < v.D)
-            *(float4*)(row + d + 4) =
-                make_float4(y[8 * h + 4], y[8 * h + 5], y[8 * h + 6], y[8 * h + 7]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (d + j < v.D) row[d + j] = y[8 * h + j];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int pos = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-        if (pos < lo || pos >= len) continue;
-        float* row = dst + (int64_t)(row0 + pos - start) * stride;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (32 * c + 16 * h + i < v.D) row[32 * c + 16 * h + i] = y[8 * h + j];
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int t = t0 + 16 * h + i;
+      if (t < lo || t >= len) continue;
+      const uint32_t w0 = h ? w.z : w.x, w1 = h ? w.w : w.y;
+      store_four(row(t), d, D, vec,
+                 make_float4(code_of(w0, 0) * s, code_of(w0, 1) * s, code_of(w0, 2) * s,
+                             code_of(w0, 3) * s));
+      store_four(row(t), d + 4, D, vec,
+                 make_float4(code_of(w1, 0) * s, code_of(w1, 1) * s, code_of(w1, 2) * s,
+                             code_of(w1, 3) * s));
     }
+  } else {
+    // elements 4 e .. 4 e + 3 of the tile, tokens t .. t + 3
+    const int e = lane & 7, q = lane >> 3, g = q & 3;
+    const int d = 32 * c + 4 * e, t = t0 + 16 * (q >> 2) + 4 * g;
+    const int8_t* x = tile + 256 * g + 16 * (4 * e & 15) + 8 * (e >> 2) + 4 * (q >> 2);
+    uint32_t w[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) w[n] = *(const uint32_t*)(x + 16 * n);
+    const float s = page < 0 ? __builtin_nanf("") : *sc;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (t + n >= lo && t + n < len)
+        store_four(row(t + n), d, D, vec,
+                   make_float4(code_of(w[0], n) * s, code_of(w[1], n) * s, code_of(w[2], n) * s,
+                               code_of(w[3], n) * s));
   }
 }
 
@@ -775,8 +787,8 @@ int plh_kv8_fetch(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int laye
                  check_rows(what, "v", v, H, D, v_stride)))
     return -1;
   a.k = k, a.vv = v, a.k_stride = k_stride, a.v_stride = v_stride;
-  a.k_vec = quads(k, k_stride, D);
-  a.groups = (2 * H + 3) / 4;
+  a.k_vec = quads(k, k_stride, D), a.v_vec = quads(v, v_stride, D);
+  a.groups = (2 * H * kv_tiles(D) + 3) / 4;
   a.fd_groups = make_fastdiv((uint32_t)a.groups);
   const int64_t wgs = kv_slots(n_rows, seqs->n_seqs) * a.groups;
   if (wgs > kMaxWorkgroups) {
