@@ -508,8 +508,9 @@ int plh_kv8_append(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, int lay
  * enter the matrix cores as two fp16 parts (22 bits).  A row before position 0
  * gets zeros; a row whose keys lie on a page number outside the cache, or in a
  * block whose scale is NaN, gets NaN.  out must not overlap q.  The partial
- * results of long sequences split over workgroups use the library workspace;
- * the first call of a head size allocates it. */
+ * results of long sequences split over workgroups use the library workspace,
+ * which a call of the same head_dim, n_rows and n_heads over as many
+ * sequences sizes before a graph is captured (lengths may differ). */
 int plh_kv8_attn(const plh_kv8_cache *cache, const plh_kv8_seqs *seqs, int layer, int n_heads,
                  int n_rows, const int32_t *row_start, const float *q, int q_stride, float *out,
                  int out_stride);

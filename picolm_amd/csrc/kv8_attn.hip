@@ -51,7 +51,7 @@ constexpr int kMinChunk = 16;      // blocks (a SHARE unit: for each of a wave's
 constexpr int kMaxTarget = 2048;   // most chunks asked for of the units that are cut
 
 // Arrival counters of cut units, zero between launches.
-__device__ unsigned g_kv8_ctr[4 * kMaxTarget];
+__device__ unsigned g_kv8_ctr[3 * kMaxTarget];
 
 struct AttnArgs {
   KvView v;
@@ -201,8 +201,10 @@ __device__ __forceinline__ void place_unit(const AttnArgs& a, Unit& u, int local
 }
 
 // Workgroup `wg`'s unit.  The quota is all units' work over the target, so at most
-// target + units workgroups have work, and the chunks of cut units, each of more
-// than half a quota, are at most 4 target.
+// target + units workgroups have work.  A unit that is cut has more blocks than a
+// chunk and so fewer than twice as many chunks as quotas of work; rounding a SHARE
+// unit's quota down to blocks (16 and more) adds a sixteenth: cut units' chunks are
+// below 3 target.
 template <int CT, bool MIXED>
 __device__ __forceinline__ Unit find_unit(const AttnArgs& a, int wg, PlanLds& lds) {
   const KvView& v = a.v;
@@ -999,7 +1001,7 @@ int launch_attn(AttnArgs& a, int n_heads, int tiles) {
   a.target = min((tiles == 2 ? 2 : 1) * waves_per_simd(DT, tiles) * ctx().num_cus, kMaxTarget);
   a.per_target = nextafterf(1.0f / (float)a.target, 1.0f);
   a.part_cols = uc;
-  if (ensure_workspace((size_t)4 * a.target * uc * Sizes<DT>::kRow * sizeof(float))) return -1;
+  if (ensure_workspace((size_t)3 * a.target * uc * Sizes<DT>::kRow * sizeof(float))) return -1;
   a.part = (float*)ctx().ws;
   // The kernel's own plan has at most target + units workgroups with work, and no
   // unit more chunks than its table row can fill.  (A sequence's units are at most

@@ -163,6 +163,44 @@ def test_many_sequences(gpu, n_seqs):
     check_attention(gpu, ref, 3, some, n_seqs + 1)
 
 
+# Launches of many units (from two for every CU on) give a wave two tiles of columns:
+# kv heads enough for that at any number of CUs up to 256.
+
+
+@pytest.mark.parametrize("D", [2, 32, 50, 64, 80, 96, 128, 144, 192, 208, 256])
+def test_wide_units_of_every_head_size(gpu, D):
+    lens, rows = [230, 90, 40, 33, 7], [200, 70, 33, 2, 1]
+    ref = make(1, 128, D, 32, lens, D)
+    print(f"[case] wide units D {D}", flush=True)
+    check_attention(gpu, ref, 128, rows, D)
+
+
+@pytest.mark.parametrize("case", [(64, 64, 3, [1900, 2500, 31]), (128, 96, 2, [1100, 2100, 1]),
+                                  (80, 128, 1, [1300, 700, 400])])
+def test_wide_units_over_long_contexts(gpu, case):
+    """Their chunks' partial results joined."""
+    D, H, G, lens = case
+    rows = [150, 65, 1]
+    ref = make(1, H, D, 64, lens, D)
+    # two units for each of 256 CUs
+    assert sum(rows) * H * G // 128 + 3 * H >= 2 * 256
+    print(f"[case] wide units {case}", flush=True)
+    out = check_attention(gpu, ref, H * G, rows, D)
+    assert np.array_equal(out, check_attention(gpu, ref, H * G, rows, D))
+
+
+@pytest.mark.parametrize("n_seqs", [64, 65, 300])
+def test_wide_units_of_many_sequences(gpu, n_seqs):
+    rng = np.random.default_rng(n_seqs)
+    lens = [int(x) for x in rng.integers(0, 200, n_seqs)]
+    lens[5] = 1500
+    ref = make(1, 8, 32, 32, lens, n_seqs)
+    rows = [int(x) if n >= x else 0 for n, x in zip(lens, rng.integers(0, 60, n_seqs))]
+    rows[5] = 300
+    print(f"[case] wide units, sequences {n_seqs}", flush=True)
+    check_attention(gpu, ref, 16, rows, n_seqs)
+
+
 def test_rows_before_position_zero(gpu):
     """More rows than tokens: the first ones see nothing and give zeros."""
     for rows, lens in (([5, 3, 200], [2, 0, 150]), ([1, 1, 1], [0, 0, 1])):
