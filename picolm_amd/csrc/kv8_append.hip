@@ -78,8 +78,7 @@ struct AppendArgs {
   int block_wgs;   // workgroups of the slots; those behind them rotate q rows
   int q_rows;      // rows of such a workgroup (1..kQRows)
   int rope;        // rotate
-  int k_vec;         // float4 reads of k rows
-  int tab_vec, half_vec;  // ... of the tables; of a k row's partners too
+  int k_vec;       // float4 reads of k rows and tables
   RopeRows r;      // the tables, and q
 };
 
@@ -121,9 +120,9 @@ __device__ __forceinline__ void here(float (&x)[N]) {
 }
 
 // N elements of a row from d on, inside it (D elements) whatever d is.
-template <int N>
-__device__ __forceinline__ void load_n(const float* row, int d, int D, int vec, float (&x)[N]) {
-  if (vec) {
+template <int N, bool VEC>
+__device__ __forceinline__ void load_n(const float* row, int d, int D, float (&x)[N]) {
+  if (VEC) {
 #pragma unroll
     for (int n = 0; n < N; n += 4) {
       const float4 a = *(const float4*)(row + min(d + n, D - 4));
@@ -135,14 +134,16 @@ __device__ __forceinline__ void load_n(const float* row, int d, int D, int vec, 
   }
 }
 
-// What turns a k row's elements 32 (c0 + t) + 8 g + j: the tables' entries and, in
-// half-split pairs, the elements' partners.
-template <int N, int MODE>
+// What turns a k row's elements 32 (c0 + t) + e .. + 3: the tables' entries and, in
+// half-split pairs, the elements' partners.  VEC: half of the rotated part is a
+// multiple of 4, so that all four lie on one side of it.  (Without branches: the
+// compiler otherwise waits for one element's loads before it asks for the next's.)
+template <int N, int MODE, bool VEC>
 struct Turn {
-  float y[N][8], c[N][8], s[N][8];
+  float y[N][4], c[N][4], s[N][4];
   bool known;
 
-  __device__ __forceinline__ void load(const AppendArgs& a, const float* row, int c0, int g,
+  __device__ __forceinline__ void load(const AppendArgs& a, const float* row, int c0, int e,
                                        int pos) {
     const int rot = a.r.rot, half = rot / 2;
     known = pos < a.r.n_pos;
@@ -151,39 +152,52 @@ struct Turn {
     const float* sin_t = a.r.sin_t + tab;
 #pragma unroll
     for (int t = 0; t < N; ++t) {
-      const int d = 32 * (c0 + t) + 8 * g;
-      if (MODE == LLAMA) {
-        float c4[4], s4[4];
-        load_n(cos_t, d / 2, half, a.tab_vec, c4);
-        load_n(sin_t, d / 2, half, a.tab_vec, s4);
+      const int d = 32 * (c0 + t) + e;
+      if (MODE == LLAMA && VEC) {
+        const int k = min(d / 2, half - 2);
+        const float2 c2 = *(const float2*)(cos_t + k), s2 = *(const float2*)(sin_t + k);
+        c[t][0] = c2.x, c[t][1] = c2.y, s[t][0] = s2.x, s[t][1] = s2.y;
+      } else if (MODE == LLAMA) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[t][j] = c4[j], s[t][j] = s4[j];
-      } else if (a.half_vec) {  // half is a multiple of 8: all eight on one side of it
-        const int e = min(d, rot - 8);
-        const bool lo = e < half;
-        load_n(row, lo ? e + half : e - half, a.v.D, 1, y[t]);
-        load_n(cos_t, lo ? e : e - half, half, 1, c[t]);
-        load_n(sin_t, lo ? e : e - half, half, 1, s[t]);
+        for (int j = 0; j < 2; ++j) {
+          const int k = min(d / 2 + j, half - 1);
+          c[t][j] = cos_t[k], s[t][j] = sin_t[k];
+        }
+      } else if (VEC) {
+        const int k = min(d, rot - 4);
+        const bool lo = k < half;
+        load_n<4, true>(row, lo ? k + half : k - half, a.v.D, y[t]);
+        load_n<4, true>(cos_t, lo ? k : k - half, half, c[t]);
+        load_n<4, true>(sin_t, lo ? k : k - half, half, s[t]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int e = min(d + j, rot - 1), k = e < half ? e : e - half;
-          y[t][j] = row[e < half ? e + half : e - half];
+        for (int j = 0; j < 4; ++j) {
+          const int f = min(d + j, rot - 1), k = f < half ? f : f - half;
+          y[t][j] = row[f < half ? f + half : f - half];
           c[t][j] = cos_t[k], s[t][j] = sin_t[k];
         }
       }
     }
   }
+  __device__ __forceinline__ void stay() {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int j = 0; j < (MODE == LLAMA ? 2 : 4); ++j) {
+        if (MODE == QWEN) asm volatile("" : "+v"(y[t][j]));
+        asm volatile("" : "+v"(c[t][j]), "+v"(s[t][j]));
+      }
+  }
 
-  __device__ __forceinline__ void apply(const AppendArgs& a, int c0, int g, float (&x)[N][8]) {
+  __device__ __forceinline__ void apply(const AppendArgs& a, int c0, int e, float (&x)[N][4]) {
     const int rot = a.r.rot, half = rot / 2;
     const float nan = __builtin_nanf("");
 #pragma unroll
     for (int t = 0; t < N; ++t) {
-      const int d = 32 * (c0 + t) + 8 * g;
+      const int d = 32 * (c0 + t) + e;
       if (MODE == LLAMA) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           float x0 = x[t][2 * j], x1 = x[t][2 * j + 1];
           rotate_pair(x0, x1, known ? c[t][j] : nan, known ? s[t][j] : nan);
           const bool in = d + 2 * j < rot;
@@ -191,14 +205,14 @@ struct Turn {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
           // (the pair's output that this element is: rotate_pair's bits, as products
           // of two fp32 values are exact)
-          const int e = d + j;
-          const double sn = known ? (e < half ? -s[t][j] : s[t][j]) : nan;
+          const int f = d + j;
+          const double sn = known ? (f < half ? -s[t][j] : s[t][j]) : nan;
           const double cs = known ? c[t][j] : nan;
           const float r = (float)__builtin_fma((double)x[t][j], cs, (double)y[t][j] * sn);
-          x[t][j] = e >= rot ? x[t][j] : r;
+          x[t][j] = f >= rot ? x[t][j] : r;
         }
       }
     }
@@ -358,13 +372,46 @@ struct Share {
   static constexpr int kJobs = 4 / kWaves;                        // of a workgroup
 };
 
+// Elements e + j of tokens 8 n + u of a k block's tiles c0.., rotated, as x[t][4 n + j].
+// ask: what else is asked for meanwhile.
+template <int T, int MODE, bool VEC, class Ask>
+__device__ __forceinline__ void k_values(const AppendArgs& a, const Place& p, int c0, int e, int u,
+                                         Ask ask, float (&x)[T][16]) {
+  float y[4][T][4];
+  Turn<T, MODE, VEC> turn[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int at = min(max(p.t0 + 8 * n + u, p.lo), p.len - 1);
+    const float* row = a.k + (int64_t)(p.row0 + at - p.start) * a.k_stride + p.head * a.v.D;
+#pragma unroll
+    for (int t = 0; t < T; ++t) load_n<4, VEC>(row, 32 * (c0 + t) + e, a.v.D, y[n][t]);
+    if (MODE != PLAIN) turn[n].load(a, row, c0, e, at);
+  }
+  ask();
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) here(y[n][t]);
+    if (MODE != PLAIN) turn[n].stay();
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    if (MODE != PLAIN) turn[n].apply(a, c0, e, y[n]);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[t][4 * n + j] = y[n][t][j];
+  }
+}
+
 // Several new rows: a wave's tiles of them in registers in the order of the codes (so
 // each lane ends with 16 adjacent bytes of every tile); the waves of a job
 // exchange their largest magnitudes.  Blocks with older rows read their tiles and
 // put them back whole.
 template <int DT, int MODE>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p, bool active,
-                                            const int32_t* entry, int b, float* red) {
+                                            const int32_t* entry, int b, float* red,
+                                            uint32_t (*turned)[256]) {
   constexpr int T = Share<DT>::kTiles;
   const KvView& v = a.v;
   const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
@@ -395,44 +442,21 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p,
         if (c0 + t < DT) old[t] = tiles[(c0 + t) * 64 + lane];
     }
   };
-  // x[t][8 h + j]: the element whose code is byte 8 h + j of this lane's sixteen of
-  // tile c0 + t (rows that are not new: a new one's, not used)
+  // v: x[t][8 h + j] is the element whose code is byte 8 h + j of this lane's sixteen of
+  // tile c0 + t.  k: x[t][4 n + j] is element e + j of token 8 n + u, so that eight lanes
+  // read 128 bytes of a row and of the tables, and the codes change lanes through LDS.
+  // (In the codes' order neighbouring lanes have different rows: 64 cache accesses a
+  // load, which bound it; 5000 rows of 8 heads of 128, half-split pairs, took 55 us.)
+  // Rows that are not new: a new one's, not used.
   float x[T][16];
   float amax = 0.0f;
+  const int e = 4 * (lane & 7), u = lane >> 3;
   if (!active) {
   } else if (!p.is_v) {
-    float y[2][T][8];
-    const float* row[2];
-    int at[2];
-    Turn<T, MODE> turn[2];
-    const bool turns = MODE != PLAIN && 32 * c0 < a.r.rot;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int pos = p.t0 + 16 * h + i;
-      at[h] = min(max(pos, p.lo), p.len - 1);
-      row[h] = a.k + (int64_t)(p.row0 + at[h] - p.start) * a.k_stride + p.head * v.D;
-#pragma unroll
-      for (int t = 0; t < T; ++t) load_n(row[h], 32 * (c0 + t) + 8 * g, v.D, a.k_vec, y[h][t]);
-    }
-    // (half-split pairs take three times the registers: one token at a time)
-    if (turns) turn[0].load(a, row[0], c0, g, at[0]);
-    if (turns && MODE == LLAMA) turn[1].load(a, row[1], c0, g, at[1]);
-    ask();
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int t = 0; t < T; ++t) here(y[h][t]);
-    if (turns) {
-      turn[0].apply(a, c0, g, y[0]);
-      if (MODE == QWEN) turn[1].load(a, row[1], c0, g, at[1]);
-      turn[1].apply(a, c0, g, y[1]);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[t][8 * h + j] = y[h][t][j];
+    if (a.k_vec)
+      k_values<T, MODE, true>(a, p, c0, e, u, ask, x);
+    else
+      k_values<T, MODE, false>(a, p, c0, e, u, ask, x);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -455,7 +479,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p,
       if (c + 32 > v.D) {  // elements behind D
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
-          const int d = p.is_v ? c + 16 * (n >> 3) + i : c + 8 * g + (n & 7);
+          const int d = c + (p.is_v ? 16 * (n >> 3) + i : e + (n & 3));
           x[t][n] = d < v.D ? x[t][n] : 0.0f;
         }
       }
@@ -480,9 +504,9 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p,
   for (int h = 0; h < 2; ++h) {
     mask[h] = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int u = p.t0 + 16 * h + (p.is_v ? 4 * g + e : i);
-      mask[h] |= u >= p.lo && u < p.len ? 0xFFu << (8 * e) : 0u;
+    for (int b8 = 0; b8 < 4; ++b8) {
+      const int pos = p.t0 + 16 * h + (p.is_v ? 4 * g + b8 : i);
+      mask[h] |= pos >= p.lo && pos < p.len ? 0xFFu << (8 * b8) : 0u;
     }
   }
 #pragma unroll
@@ -492,6 +516,16 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p,
     const uint32_t k4[4] = {kept.x, kept.y, kept.z, kept.w};
     uint32_t w[4];
     codes16(x[t], s, w);
+    if (!p.is_v) {
+      // w[n] is bytes e & 7 .. of token 8 n + u (the wave's own 1024 bytes)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        turned[wave][64 * (e >> 3) + 4 * ((8 * n + u) & 15) + 2 * (n >> 1) + ((e & 7) >> 2)] = w[n];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = turned[wave][4 * lane + q];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const uint32_t m = p.is_v ? mask[q & 1] : mask[q >> 1];
@@ -519,6 +553,7 @@ template <int DT, int MODE>
 __global__ __launch_bounds__(kKvThreads, DT > 4 ? 2 : MODE == QWEN ? 5 : 6) void
 kv8_append_kernel(AppendArgs a) {
   __shared__ float red[4];
+  __shared__ __align__(16) uint32_t turned[4][256];
   const KvView& v = a.v;
   if (MODE != PLAIN && (int)blockIdx.x >= a.block_wgs) {
     const int wg = (int)blockIdx.x - a.block_wgs;
@@ -563,7 +598,7 @@ kv8_append_kernel(AppendArgs a) {
   const int e = (int)fdiv((uint32_t)k.block, v.fd_blocks), b = k.block - e * v.blocks;
   const int32_t* entry = v.table + (size_t)k.s * v.max_pages + e;
   if (min(p.len, p.t0 + kKvBlock) - max(p.lo, p.t0) > 1) {
-    append_rows<DT, MODE>(a, p, active, entry, b, red);
+    append_rows<DT, MODE>(a, p, active, entry, b, red, turned);
     return;
   }
   if (!active || wave % Share<DT>::kWaves) return;
@@ -767,8 +802,7 @@ int plh_kv8_append(const plh_kv8_cache* cache, const plh_kv8_seqs* seqs, int lay
     a.r = rope_rows_args(rope, D, q, n_heads, q_stride, q_out, q_out_stride, nullptr, 0, 0,
                          nullptr, 0);
     const bool tab16 = (((uintptr_t)rope->cos_tab | (uintptr_t)rope->sin_tab) & 15) == 0;
-    a.tab_vec = tab16 && rope->rot_dim % 8 == 0;
-    a.half_vec = tab16 && a.k_vec && rope->rot_dim % 16 == 0;
+    a.k_vec = a.k_vec && tab16 && rope->rot_dim % 8 == 0;
   }
   a.block_wgs = (int)(wgs < INT_MAX ? wgs : INT_MAX);
   // Prompts: several rows' loads in flight a workgroup; while there are few rows,
