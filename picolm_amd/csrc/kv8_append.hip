@@ -446,7 +446,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p,
   // tile c0 + t.  k: x[t][4 n + j] is element e + j of token 8 n + u, so that eight lanes
   // read 128 bytes of a row and of the tables, and the codes change lanes through LDS.
   // (In the codes' order neighbouring lanes have different rows: 64 cache accesses a
-  // load, which bound it; 5000 rows of 8 heads of 128, half-split pairs, took 55 us.)
+  // load, which bound it: 5000 rows of 8 heads of 128, half-split pairs, took 55 us
+  // and take 14.)
   // Rows that are not new: a new one's, not used.
   float x[T][16];
   float amax = 0.0f;
@@ -543,12 +544,12 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Place& p,
 // HBM bounds prompts (4 bytes read and 1 written an element); single tokens are
 // three memory latencies: row_start with len, the row with the page number, the
 // page's count and scale.  4870 prompt rows with 32 q heads and 8 kv heads of 64
-// take 26 us (100 MB, 3.8 TB/s; 12 without q); 64 single tokens with 16 and 8 heads
-// of 128 take 5 us; 872 rows of 32 and 32 heads of 80 take 19 us, where the waves
-// come in five rounds of these latencies (40 MB, 9 us at a large copy's rate).
+// take 24 us (100 MB, 4.2 TB/s; 9.4 without q); 64 single tokens with 16 and 8 heads
+// of 128 take 6 us; 872 rows of 32 and 32 heads of 80 take 14 us, two or three rounds
+// of these latencies (40 MB, 9 us at a large copy's rate).
 //
 // A wave a tile, so that a job's loads are few and together: with whole jobs a wave
-// the last of these took 27 us.
+// the last of these took 1.4 times as long.
 template <int DT, int MODE>
 __global__ __launch_bounds__(kKvThreads, DT > 4 ? 2 : MODE == QWEN ? 5 : 6) void
 kv8_append_kernel(AppendArgs a) {
@@ -565,7 +566,7 @@ kv8_append_kernel(AppendArgs a) {
 #pragma unroll
     for (int n = 0; n < kQRows; ++n) {
       const int64_t row = (int64_t)group * a.q_rows + n;
-      if (n < a.q_rows && row < v.n_rows && item < a.r.per_row) 
+      if (n < a.q_rows && row < v.n_rows && item < a.r.per_row)
         it[n] = rope_load<MODE == QWEN>(a.r, row, item);
     }
 #pragma unroll
@@ -632,12 +633,11 @@ __device__ __forceinline__ void store_four(float* row, int d, int D, int vec, fl
   }
 }
 
-// A wave per block, kv head, k or v and tile.  Of k a lane takes 16 adjacent bytes,
-// eight elements of two tokens; of v four words, four elements of four tokens: rows
-// are written 128 bytes at a time.  HBM (the 4-byte values written) bounds it, or for
-// few rows the latencies of lengths, page, codes and stores: 2 K rows of 8 heads of
-// 128 (17 MB written) take 8 us; with whole heads a wave and v stored by single
-// elements it was 9.3.
+// A wave per block, kv head, k or v and tile; a lane's four words are chosen so that
+// rows are written 128 bytes at a time by eight neighbouring lanes.  HBM (the 4-byte
+// values written) bounds it, or for few rows the latencies of lengths, page, codes and
+// stores: 2 K rows of 8 heads of 128 (17 MB written) take 8 us; with a whole head a
+// wave it was 9.3.
 template <int DT>
 __global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
   const KvView& v = a.v;
@@ -666,38 +666,29 @@ __global__ __launch_bounds__(kKvThreads) void kv8_fetch_kernel(FetchArgs a) {
   const int8_t* tile = v.codes + src * v.page_codes + ((int64_t)unit * DT + c) * kKvTile;
   const float* sc = v.scales + src * v.page_scales + unit;
   const int t0 = blk * kKvBlock;
-  auto row = [&](int t) { return dst + (int64_t)(row0 + t - start) * stride; };
+  // A lane's four words: of k elements d .. d + 3 of tokens t, t + 8, .., of v elements
+  // d .. d + 3, each of tokens t .. t + 3.
+  const int e = lane & 7, q = lane >> 3, d = 32 * c + 4 * e;
+  uint32_t w[4];
   if (!is_v) {
-    const int g = lane >> 4, i = lane & 15, d = 32 * c + 8 * g;
-    const uint4 w = ((const uint4*)tile)[lane];
-    const float s = page < 0 ? __builtin_nanf("") : *sc;
+    const int8_t* x = tile + 256 * (e >> 1) + 4 * (e & 1) + 16 * q;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = t0 + 16 * h + i;
-      if (t < lo || t >= len) continue;
-      const uint32_t w0 = h ? w.z : w.x, w1 = h ? w.w : w.y;
-      store_four(row(t), d, D, vec,
-                 make_float4(code_of(w0, 0) * s, code_of(w0, 1) * s, code_of(w0, 2) * s,
-                             code_of(w0, 3) * s));
-      store_four(row(t), d + 4, D, vec,
-                 make_float4(code_of(w1, 0) * s, code_of(w1, 1) * s, code_of(w1, 2) * s,
-                             code_of(w1, 3) * s));
-    }
+    for (int n = 0; n < 4; ++n) w[n] = *(const uint32_t*)(x + 128 * (n & 1) + 8 * (n >> 1));
   } else {
-    // elements 4 e .. 4 e + 3 of the tile, tokens t .. t + 3
-    const int e = lane & 7, q = lane >> 3, g = q & 3;
-    const int d = 32 * c + 4 * e, t = t0 + 16 * (q >> 2) + 4 * g;
-    const int8_t* x = tile + 256 * g + 16 * (4 * e & 15) + 8 * (e >> 2) + 4 * (q >> 2);
-    uint32_t w[4];
+    const int8_t* x = tile + 256 * (q & 3) + 16 * (4 * e & 15) + 8 * (e >> 2) + 4 * (q >> 2);
 #pragma unroll
     for (int n = 0; n < 4; ++n) w[n] = *(const uint32_t*)(x + 16 * n);
-    const float s = page < 0 ? __builtin_nanf("") : *sc;
+  }
+  const float s = page < 0 ? __builtin_nanf("") : *sc;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (t + n >= lo && t + n < len)
-        store_four(row(t + n), d, D, vec,
-                   make_float4(code_of(w[0], n) * s, code_of(w[1], n) * s, code_of(w[2], n) * s,
-                               code_of(w[3], n) * s));
+  for (int n = 0; n < 4; ++n) {
+    const int t = t0 + (is_v ? 16 * (q >> 2) + 4 * (q & 3) + n : 8 * n + q);
+    if (t < lo || t >= len) continue;
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (is_v ? code_of(w[j], n) : code_of(w[n], j)) * s;
+    store_four(dst + (int64_t)(row0 + t - start) * stride, d, D, vec,
+               make_float4(y[0], y[1], y[2], y[3]));
   }
 }
 

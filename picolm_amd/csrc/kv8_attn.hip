@@ -445,7 +445,8 @@ struct Columns {
                               vmax(vmax(s1[ct][0], s1[ct][1]), vmax(s1[ct][2], s1[ct][3])));
       above = vmax(above, __builtin_fmaf(top8, f[ct], -thr[ct]));
     }
-    const bool unit_fits = (ve - d_hi >= kUnitLo && ve - d_lo <= kUnitHi) || __builtin_amdgcn_readfirstlane(vs == 0.0f);
+    const bool unit_fits = (ve - d_hi >= kUnitLo && ve - d_lo <= kUnitHi) ||
+                           __builtin_amdgcn_readfirstlane(vs == 0.0f);
     if (!seen_whole || !unit_fits || !__all(above <= 0.0f)) {
       far = false, d_lo = INT_MAX, d_hi = INT_MIN;
 #pragma unroll

@@ -153,10 +153,11 @@ constexpr int kListed = 4096;  // free pages kept in LDS; more go to the workspa
 
 // extend: a thread per sequence finds what it needs, all of them walk refs
 // for the free pages of the lowest numbers until there are enough, and if so
-// hand them out (5.1 us for 18 sequences).  One workgroup: the walk is 16 KB a step and ends early; a
-// pool of 64 K pages with its free ones last takes 16 steps.  Few sequences on
-// few pages (a decode step) are four memory latencies and two barriers: wish,
-// len and the first 4096 counts together; last pages; their counts; stores.
+// hand them out (5.1 us for 18 sequences).  One workgroup: the walk is 16 KB a
+// step and ends early; a pool of 64 K pages with its free ones last takes 16
+// steps.  Few sequences on few pages (a decode step) are four memory latencies
+// and two barriers: wish, len and the first 4096 counts together; last pages;
+// their counts; stores.
 __global__ __launch_bounds__(kPlanThreads) void kv8_extend_kernel(PageArgs a) {
   __shared__ int32_t last[kKvMaxSeqs], at[kKvMaxSeqs], from[kKvMaxSeqs], to[kKvMaxSeqs];
   __shared__ int32_t list[kListed];
@@ -327,7 +328,8 @@ __global__ __launch_bounds__(kKvThreads) void kv8_copy_kernel(PageArgs a, int re
   int c = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - c * a.chunks;
   while (c < n) {
     const int64_t from = a.src[c], to = a.dst[c];
-    const uint32_t at = (uint32_t)chunk * kCopyChunk + threadIdx.x * 16, end = (uint32_t)a.page_codes;
+    const uint32_t at = (uint32_t)chunk * kCopyChunk + threadIdx.x * 16;
+    const uint32_t end = (uint32_t)a.page_codes;
     const int8_t* x = a.codes + from * a.page_codes + at;
     int8_t* y = a.codes + to * a.page_codes + at;
     Vec16 r[kCopyLoads];
