@@ -73,16 +73,18 @@ __device__ __forceinline__ KvLanes kv_lanes(const KvView& v) {
   return l;
 }
 // The number of sequences i for which before(i, row_start[i + 1]) holds: with
-// row_start rising, the first sequence for which it does not (n_seqs: none).
+// row_start rising, the first sequence for which it does not (n_seqs: none).  More
+// than 64: the last of each 64th part first, then the part where it ends.
 template <class F>
 __device__ __forceinline__ int kv_find(const KvView& v, const KvLanes& l, F before) {
-  const int lane = (int)threadIdx.x & 63;
-  int s = __popcll(__ballot(lane < v.n_seqs && before(lane, l.next)));
-  for (int at = 64; at < v.n_seqs; at += 64) {
-    const int i = at + lane;
-    s += __popcll(__ballot(i < v.n_seqs && before(i, v.row_start[min(i, v.n_seqs - 1) + 1])));
-  }
-  return s;
+  const int lane = (int)threadIdx.x & 63, n = v.n_seqs;
+  if (n <= 64) return __popcll(__ballot(lane < n && before(lane, l.next)));
+  const int per = (n + 63) / 64;
+  int i = min((lane + 1) * per, n) - 1;
+  const int at = per * __popcll(__ballot(lane * per < n && before(i, v.row_start[i + 1])));
+  i = min(at + lane, n - 1);
+  const bool mine = lane < per && at + lane < n;
+  return min(at + (int)__popcll(__ballot(mine && before(i, v.row_start[i + 1]))), n);
 }
 // Rows (as kv_rows) and tokens of sequence s, from the lanes where they hold it.
 struct KvSeq {
