@@ -571,6 +571,46 @@ def test_q_rows_behind_the_tables_and_sequences(gpu):
     dev.free()
 
 
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("case", [(3, 1400), (70, 60), (65, 1), (300, 2), (1024, 5)])
+def test_append_many_rows_and_sequences(gpu, case, kind):
+    """Few and many sequences, rows enough that a workgroup takes several q rows; q
+    is rotated in place, and everything is read back."""
+    n_seqs, rows = case
+    P, D = gpu, 32
+    rng = np.random.default_rng(n_seqs + kind)
+    rows = [int(x) for x in rng.integers(max(rows - 8, 0), rows + 1, n_seqs)]
+    lens = [m + int(x) for m, x in zip(rows, rng.integers(0, 40, n_seqs))]
+    n = sum(rows)
+    ref = make(1, 2, D, 64, lens, n_seqs)
+    dev = Dev(P, ref)
+    n_pos = max(lens)
+    angle = rng.uniform(-4, 4, (n_pos, 12))
+    tabs = [P.DeviceBuffer.from_numpy(f(angle).astype(np.float32)) for f in (np.cos, np.sin)]
+    rope = P.rope.Tables(kind, 24, n_pos, tabs[0].ptr, tabs[1].ptr)
+    k, v = (rng.normal(size=(n, 2, D)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(n, 3, D)).astype(np.float32)
+    pos = np.concatenate([np.arange(a - m, a) for a, m in zip(lens, rows)]).astype(np.int32)
+    print(f"[case] append {case} kind {kind}", flush=True)
+    dpos, drs = P.DeviceBuffer.from_numpy(pos), P.DeviceBuffer.from_numpy(starts(rows))
+    turned = []
+    for x in (k, q):
+        b = P.DeviceBuffer.from_numpy(x)
+        w = x.shape[1] * D
+        P.rope.rotate(rope, n, dpos.ptr, D, b.ptr, x.shape[1], w, b.ptr, w)
+        P.synchronize()
+        turned.append(b.download(np.float32, x.shape))
+    ref.append(0, starts(rows), turned[0], v)
+    dk, dv, dq = (P.DeviceBuffer.from_numpy(x) for x in (k, v, q))
+    P.kv8.append(dev.cache, dev.seqs, 0, n, drs.ptr, dk.ptr, dv.ptr, rope=rope, q=dq.ptr,
+                 n_heads=3, q_out=dq.ptr)
+    P.synchronize()
+    assert np.array_equal(dq.download(np.float32, q.shape), turned[1])
+    dev.same_contents(case)
+    check_fetch(P, dev, 0, rows)
+    dev.free()
+
+
 # ---- pages ----------------------------------------------------------------------
 
 
