@@ -676,6 +676,42 @@ def test_fork_permutes(gpu):
     dev.free()
 
 
+@pytest.mark.parametrize("shape", [(200, 50), (1024, 12), (3, 4000)])
+def test_pages_of_large_tables(gpu, shape):
+    """Forks beyond one workgroup's table, branches of one parent that all grow, ends
+    and compaction."""
+    P = gpu
+    S, width = shape
+    rng = np.random.default_rng(S)
+    n_pages = 4 * S + 3 * width
+    ref = Ref(1, 1, 32, n_pages, 32, S, width)
+    ref.codes[:] = rng.integers(-127, 128, ref.codes.shape)
+    dev = Dev(P, ref)
+    st = vec(P, [-1, -1])
+    add = np.zeros(S, np.int64)
+    add[:3] = [32 * (width - 2) + 5, 40, 7]
+    x = np.full(S, -1)
+    x[3:] = rng.integers(0, 3, S - 3)
+    shift = np.where(rng.random(S) < 0.5, rng.integers(0, S, S), -1)
+    print(f"[case] large tables {shape}", flush=True)
+    for step, (op, arg) in enumerate([("extend", add), ("fork", x), ("extend", np.ones(S, int)),
+                                      ("fork", shift), ("extend", rng.integers(0, 9, S)),
+                                      ("trim", np.where(rng.random(S) < 0.6, 0, -1)),
+                                      ("compact", None)]):
+        if op in ("extend", "compact"):
+            want = ref.extend(arg) if op == "extend" else ref.compact()
+            getattr(P.kv8, op)(dev.cache, dev.seqs, *([] if arg is None else [vec(P, arg).ptr]),
+                               st.ptr)
+            assert status(P, st) == want, step
+        else:
+            getattr(ref, op)(arg)
+            getattr(P.kv8, op)(dev.cache, dev.seqs, vec(P, arg).ptr)
+        P.synchronize()
+        dev.same_state((step, op))
+        dev.same_contents((step, op))
+    dev.free()
+
+
 @pytest.mark.parametrize("n_pages", [1, 4095, 4096, 4097, 20000])
 def test_allocation_over_many_pages(gpu, n_pages):
     """The free pages are the last ones, or every third; a request for all of them,
