@@ -73,7 +73,7 @@ struct AppendArgs {
   KvView v;
   const float *k, *vv;
   int k_stride, v_stride;
-  int groups;      // workgroups of a slot: four jobs (a head's k or v) each
+  int groups;      // workgroups of a slot: Share::kJobs jobs (a head's k or v) each
   FastDiv fd_groups;
   int block_wgs;   // workgroups of the slots; those behind them rotate q rows
   int q_rows;      // rows of such a workgroup (1..kQRows)
